@@ -346,6 +346,168 @@ MOE_API int moe_quantize_device(const float *src, int64_t rows, int64_t cols, in
 			void *dst, void *stream);
 
 /* ------------------------------------------------------------------ */
+/* Rotary positions, the paged 4-bit key/value cache, attention over it */
+/* ------------------------------------------------------------------ */
+
+/* No counterpart in the reference, whose kvcache.c holds one sequence in
+ * fp32: the attention side of a decoder block for an engine that serves
+ * many sequences.  All pointers below are device pointers unless a comment
+ * says host; every call is asynchronous on `stream` (NULL = the library
+ * stream, (void *)1 = CUDA's legacy default stream), may be recorded into a
+ * CUDA graph, allocates nothing, and runs on the device that its handle was
+ * created on, whichever is current.  A call that returns an error status has
+ * launched nothing.  Calls that may overlap on the GPU need workspaces of
+ * their own and must not write the same rows. */
+
+/* element types of activations beside MOE_F32 (outside the reference's enum) */
+enum { MOE_F16 = 16, MOE_BF16 = 17 };
+
+/* Heads of a packed batch of tokens: value e of head h of token t is
+ * data[t * token_stride + h * head_stride + e] (strides in elements), e.g. the
+ * Q, K or V part of a fused projection's rows.  An input's strides may be 0 (one
+ * row for all); an output's rows must not overlap. */
+typedef struct moe_rows {
+	void *data;
+	int type;                      /* MOE_F32, MOE_F16 or MOE_BF16      */
+	int64_t n_heads, token_stride, head_stride;
+} moe_rows;
+
+/* which values of a head turn together: 2i and 2i + 1 (the reference's
+ * rope_apply, nn.c:192-219), or i and i + rot / 2 */
+enum { MOE_ROPE_PAIRS = 0, MOE_ROPE_HALVES = 1 };
+/* frequency scaling for contexts longer than the trained one; f_i =
+ * theta^(-2i / rot) radians a position for pair i:
+ *   NONE    f_i
+ *   LINEAR  f_i / factor
+ *   PARTS   f_i / factor * r + f_i * (1 - r): r ramps from 0 to 1 between the
+ *           pairs floor(p(beta_fast)) and ceil(p(beta_slow)), p(n) the pair
+ *           that makes n turns over orig_context positions (held to [0, rot - 1])
+ *   BANDS   (1 - s) f_i / factor + s f_i, s = (turns_i - low_freq) /
+ *           (high_freq - low_freq) held to [0, 1], turns_i the pair's turns over
+ *           orig_context positions */
+enum { MOE_ROPE_NONE = 0, MOE_ROPE_LINEAR = 1, MOE_ROPE_PARTS = 2, MOE_ROPE_BANDS = 3 };
+
+typedef struct moe_rope moe_rope; /* opaque: angle tables in HBM */
+
+typedef struct moe_rope_desc {
+	int64_t rot;                   /* values of a head that turn: even    */
+	int64_t max_position;          /* positions are 0 .. max_position - 1 */
+	int layout, scaling;
+	double theta, factor;
+	double orig_context;           /* PARTS, BANDS                        */
+	double beta_fast, beta_slow;   /* PARTS (32 and 1 where both are 0)   */
+	double low_freq, high_freq;    /* BANDS                               */
+	double magnitude;              /* factor on cosine and sine; 0: 0.1 ln
+	                                * factor + 1 for PARTS, 1 otherwise   */
+	const float *freq_divisors;    /* HOST [rot / 2] or NULL: f_i is divided
+	                                * by entry i before the scaling       */
+} moe_rope_desc;
+
+/* Angles are formed in 64 bits (position times frequency; cosine and sine
+ * rounded to fp32 once), so far positions turn as exactly as near ones.
+ * max_position <= 2^24; the tables take (1024 + max_position / 1024) * rot * 8
+ * bytes. */
+MOE_API int moe_rope_create(moe_rope **out, const moe_rope_desc *desc);
+MOE_API int moe_rope_destroy(moe_rope *rope);
+/* q_out = q turned by pos[t] and, where k is not NULL, k_out = k turned: the
+ * first rot of every head's head_len values turn, the rest are copied.  fp32
+ * arithmetic (each product and sum rounded once), rounded once to the rows'
+ * type, which is one for all four.  An output may be its own input (same data
+ * and strides); they must not overlap otherwise.  A token whose position is
+ * out of range is left unwritten and recorded (moe_rope_status). */
+MOE_API int moe_rope_forward(moe_rope *rope, int64_t n_tokens, int64_t head_len, const int32_t *pos,
+			     const moe_rows *q, const moe_rows *q_out, const moe_rows *k,
+			     const moe_rows *k_out, void *stream);
+/* Waits for the device; MOE_OK, or MOE_ERR_INVALID (once) if a position was
+ * out of range since the last call. */
+MOE_API int moe_rope_status(moe_rope *rope);
+
+/* The cache of one layer: n_pages pages of page_size rows, each row the keys
+ * and values of n_kv_heads heads in 4 bits.  A row of head_len values is cut
+ * into nb = head_len / 32 blocks of 32: value = scale * (code - 8), with
+ *   scale = fp16(-m / 8), m the block's largest value or, where its magnitude is
+ *           larger, its smallest, held to +-65504 (+0 for either zero); NaN where a value of the block
+ *           is not finite (a poisoned block reads as NaN, not as a number),
+ *   code  = rint(value * (1 / scale)) + 8 held to 0 .. 15 (8 where scale is 0).
+ * Byte k of a block has the code of value k in its low nibble and of value k + 16
+ * in its high nibble, as in Q4_0.  In memory, per page and KV head:
+ *   K codes [page_size][head_len / 2], K scales [page_size][nb] fp16, V codes,
+ *   V scales alike; byte k of block b stands at byte (k / 4) * 4 nb + 4 b + k % 4
+ *   of a K row and at (k / 2) * 2 nb + 2 b + k % 2 of a V row (so that a thread of
+ *   the attention kernel finds its operands of all blocks side by side). */
+typedef struct moe_kv_cache moe_kv_cache; /* opaque */
+
+typedef struct moe_kv_desc {
+	int64_t n_pages, page_size;    /* page_size 16, 32, 64, 128 or 256    */
+	int64_t n_kv_heads, head_len;  /* head_len 64, 128 or 256             */
+	int qtype;                     /* MOE_Q4_0                            */
+	void *pages;                   /* n_pages * moe_kv_page_bytes, 16-byte
+	                                * aligned, owned by the caller; or NULL:
+	                                * allocated and zeroed                */
+} moe_kv_desc;
+
+/* bytes of one page, or 0 for a shape that is not supported */
+MOE_API size_t moe_kv_page_bytes(int64_t page_size, int64_t n_kv_heads, int64_t head_len, int qtype);
+MOE_API int moe_kv_create(moe_kv_cache **out, const moe_kv_desc *desc);
+MOE_API int moe_kv_destroy(moe_kv_cache *cache);
+/* device address of the pages */
+MOE_API void *moe_kv_pages(moe_kv_cache *cache);
+
+/* A packed batch: sequence b's rows of q, k, v are q_start[b] .. q_start[b + 1]
+ * - 1, the last of its kv_len[b] cache rows (so its query i stands at cache row
+ * kv_len[b] - n_b + i); row r of the sequence lies in page page_table[b *
+ * table_stride + r / page_size].  q_start[0] is 0; tokens from q_start[n_seqs] up
+ * to n_tokens are padding, whose outputs are left as they were.  The
+ * arrays are read on the device, so a captured call follows their contents; the
+ * four sizes are fixed by the call. */
+typedef struct moe_kv_batch {
+	int64_t n_seqs, n_tokens;      /* n_tokens: rows that q, k, v and out have */
+	int64_t max_q, max_kv;         /* bounds of n_b and of kv_len[b]      */
+	const int32_t *q_start;        /* [n_seqs + 1]                        */
+	const int32_t *kv_len;         /* [n_seqs]                            */
+	const int32_t *page_table;     /* [n_seqs][table_stride]; entries behind a
+	                                * sequence's last row are not read    */
+	int64_t table_stride;
+} moe_kv_batch;
+
+/* Appends the batch's keys and values to their rows of the cache, the keys
+ * turned on the way (rope NULL: as they are), and turns the queries (q, q_out
+ * NULL: none).  Positions are pos[t], or with pos NULL the token's cache row.
+ * k, v, q and q_out have one type; q_out may be q.  A sequence or token whose
+ * arrays, page or position are out of range is left out and recorded
+ * (moe_kv_status).  Two tokens of one call must not share a row. */
+MOE_API int moe_kv_append(moe_kv_cache *cache, const moe_kv_batch *batch, const moe_rope *rope,
+			  const int32_t *pos, const moe_rows *k, const moe_rows *v,
+			  const moe_rows *q, const moe_rows *q_out, void *stream);
+/* The batch's rows read back from the cache as the values that they stand for
+ * (k_out or v_out may be NULL).  With q_start the running sum of kv_len, whole
+ * sequences. */
+MOE_API int moe_kv_gather(moe_kv_cache *cache, const moe_kv_batch *batch, const moe_rows *k_out,
+			  const moe_rows *v_out, void *stream);
+
+/* Attention of the batch's queries over their sequences' cache rows:
+ *   out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j
+ * with k_j, v_j of KV head h / (n_heads / n_kv_heads).  With causal != 0 the query
+ * at cache row p sees rows j <= p, and with window > 0 only j > p - window
+ * (causal only; 0: all).  A query that sees no row gives zeros.  lse (fp32
+ * [n_tokens, n_heads], or NULL) receives ln sum_j exp(score), -infinity where
+ * nothing is seen.  q and out have one type.  Products take the codes exactly, q
+ * and the weights in fp16 (fp32 rows: as two fp16 halves, about 22 bits); sums
+ * and softmax statistics are fp32.  Rows that a query does not see never reach
+ * its result, whatever they hold.
+ * workspace: 16-byte aligned, at least moe_kv_attention_workspace bytes (which
+ * follow from the batch's four sizes); used by this call only. */
+MOE_API int64_t moe_kv_attention_workspace(const moe_kv_cache *cache, const moe_kv_batch *batch,
+					   int64_t n_heads);
+MOE_API int moe_kv_attention(moe_kv_cache *cache, const moe_kv_batch *batch, const moe_rows *q,
+			     const moe_rows *out, float *lse, float scale, int causal,
+			     int64_t window, void *workspace, size_t workspace_bytes, void *stream);
+/* Waits for the device; MOE_OK, or (once) MOE_ERR_INVALID if a call since the
+ * last one met arrays, pages or positions out of range, MOE_ERR_TIMEOUT if a
+ * bounded wait expired. */
+MOE_API int moe_kv_status(moe_kv_cache *cache);
+
+/* ------------------------------------------------------------------ */
 /* Whole model on the device (OLMoE, llama / Mixtral)                   */
 /* ------------------------------------------------------------------ */
 

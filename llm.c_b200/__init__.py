@@ -30,6 +30,11 @@ EP_SHARDED = 0x200
 NO_T1 = 0x400
 FORCE_T1 = 0x800
 
+# element types of packed rows beside F32, and the rotary layouts and scalings
+F16, BF16 = 16, 17
+ROPE_PAIRS, ROPE_HALVES = 0, 1
+ROPE_NONE, ROPE_LINEAR, ROPE_PARTS, ROPE_BANDS = 0, 1, 2, 3
+
 ERRORS = {0: "MOE_OK", -1: "MOE_ERR_INVALID", -2: "MOE_ERR_UNSUPPORTED", -3: "MOE_ERR_CUDA",
           -4: "MOE_ERR_NOMEM", -5: "MOE_ERR_NOT_INIT", -6: "MOE_ERR_COMM", -7: "MOE_ERR_TIMEOUT"}
 
@@ -75,11 +80,41 @@ class ModelDesc(C.Structure):
 
 ARCH_OLMOE, ARCH_LLAMA = 0, 1
 
+
+class Rows(C.Structure):
+    """moe_rows: heads of a packed batch of tokens at a device address (strides in elements)"""
+    _fields_ = [("data", C.c_void_p), ("type", C.c_int), ("n_heads", C.c_int64),
+                ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class KVBatch(C.Structure):
+    """moe_kv_batch: a packed batch of sequences; q_start, kv_len and page_table are
+    device addresses of int32 arrays"""
+    _fields_ = [("n_seqs", C.c_int64), ("n_tokens", C.c_int64), ("max_q", C.c_int64),
+                ("max_kv", C.c_int64), ("q_start", C.c_void_p), ("kv_len", C.c_void_p),
+                ("page_table", C.c_void_p), ("table_stride", C.c_int64)]
+
+
+class RopeDesc(C.Structure):
+    """moe_rope_desc"""
+    _fields_ = [("rot", C.c_int64), ("max_position", C.c_int64), ("layout", C.c_int),
+                ("scaling", C.c_int), ("theta", C.c_double), ("factor", C.c_double),
+                ("orig_context", C.c_double), ("beta_fast", C.c_double), ("beta_slow", C.c_double),
+                ("low_freq", C.c_double), ("high_freq", C.c_double), ("magnitude", C.c_double),
+                ("freq_divisors", C.POINTER(C.c_float))]
+
+
+class KVDesc(C.Structure):
+    """moe_kv_desc"""
+    _fields_ = [("n_pages", C.c_int64), ("page_size", C.c_int64), ("n_kv_heads", C.c_int64),
+                ("head_len", C.c_int64), ("qtype", C.c_int), ("pages", C.c_void_p)]
+
 _lib = None
 
 # every symbol include/moe_b200.h declares, with (restype, argtypes)
 _P, _I, _SZ, _I64, _U64, _F = C.c_void_p, C.c_int, C.c_size_t, C.c_int64, C.c_uint64, C.c_float
 _TP = C.POINTER(MoeTensor)
+_RP, _BP = C.POINTER(Rows), C.POINTER(KVBatch)
 SIGNATURES = {
     "moe_init": (_I, [_I]),
     "moe_shutdown": (_I, []),
@@ -119,6 +154,19 @@ SIGNATURES = {
     "moe_host_free": (_I, [_P]),
     "moe_synth_gauss": (_I, [_P, _U64, _U64, _U64, _I64, _F, _P]),
     "moe_quantize_device": (_I, [_P, _I64, _I64, _I, _P, _P]),
+    "moe_rope_create": (_I, [C.POINTER(_P), C.POINTER(RopeDesc)]),
+    "moe_rope_destroy": (_I, [_P]),
+    "moe_rope_forward": (_I, [_P, _I64, _I64, _P, _RP, _RP, _RP, _RP, _P]),
+    "moe_rope_status": (_I, [_P]),
+    "moe_kv_page_bytes": (_SZ, [_I64, _I64, _I64, _I]),
+    "moe_kv_create": (_I, [C.POINTER(_P), C.POINTER(KVDesc)]),
+    "moe_kv_destroy": (_I, [_P]),
+    "moe_kv_pages": (_P, [_P]),
+    "moe_kv_append": (_I, [_P, _BP, _P, _P, _RP, _RP, _RP, _RP, _P]),
+    "moe_kv_gather": (_I, [_P, _BP, _RP, _RP, _P]),
+    "moe_kv_attention_workspace": (_I64, [_P, _BP, _I64]),
+    "moe_kv_attention": (_I, [_P, _BP, _RP, _RP, _P, _F, _I, _I64, _P, _SZ, _P]),
+    "moe_kv_status": (_I, [_P]),
     "moe_model_create": (_I, [C.POINTER(_P), C.POINTER(ModelDesc)]),
     "moe_model_destroy": (_I, [_P]),
     "moe_model_prefill": (_I, [_P, _P, _P, _SZ, _P]),
@@ -477,6 +525,103 @@ def gemv(w: np.ndarray, qtype: int, rows: int, cols: int, x: np.ndarray) -> np.n
     gemv_device(bw.ptr, qtype, rows, cols, bx.ptr, x.shape[0], by.ptr)
     check(lib().moe_sync())
     return by.to_numpy(np.float32, (x.shape[0], rows))
+
+
+# ------------------------------------------------------------------ rotary positions, paged cache
+def _ref(x):
+    return None if x is None else C.byref(x)
+
+
+class Rope:
+    """Angle tables for rotary positions (moe_rope_create); scaling and its
+    parameters as moe_rope_desc describes them."""
+
+    def __init__(self, rot, theta, max_position, layout=ROPE_PAIRS, scaling=ROPE_NONE, factor=1.0,
+                 orig_context=0.0, beta_fast=0.0, beta_slow=0.0, low_freq=0.0, high_freq=0.0,
+                 magnitude=0.0, freq_divisors=None):
+        div = None
+        if freq_divisors is not None:
+            div = (C.c_float * len(freq_divisors))(*[float(f) for f in freq_divisors])
+            if len(div) != rot // 2:
+                raise MoeError(-1, f"{len(div)} frequency divisors for {rot // 2} pairs")
+        desc = RopeDesc(rot, max_position, layout, scaling, theta, factor, orig_context, beta_fast,
+                        beta_slow, low_freq, high_freq, magnitude,
+                        None if div is None else C.cast(div, C.POINTER(C.c_float)))
+        h = C.c_void_p()
+        check(lib().moe_rope_create(C.byref(h), C.byref(desc)))
+        self.handle = h.value
+
+    def forward(self, n_tokens, head_len, pos, q, q_out, k=None, k_out=None, stream=None):
+        """q_out = q (and k_out = k) turned by the device positions `pos`; Rows each"""
+        check(lib().moe_rope_forward(self.handle, n_tokens, head_len, pos, _ref(q), _ref(q_out),
+                                     _ref(k), _ref(k_out), stream))
+
+    def status(self) -> int:
+        """waits for the device; the code of moe_rope_status (0 = ok); does not raise"""
+        return lib().moe_rope_status(self.handle)
+
+    def close(self):
+        if getattr(self, "handle", None):
+            lib().moe_rope_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def kv_page_bytes(page_size, n_kv_heads, head_len, qtype=Q4_0) -> int:
+    return lib().moe_kv_page_bytes(page_size, n_kv_heads, head_len, qtype)
+
+
+class KVCache:
+    """One layer's paged key/value cache in 4 bits (moe_kv_create).  `pages`: device
+    address of the caller's n_pages * kv_page_bytes bytes, or None to allocate."""
+
+    def __init__(self, n_pages, page_size, n_kv_heads, head_len, qtype=Q4_0, pages=None):
+        desc = KVDesc(n_pages, page_size, n_kv_heads, head_len, qtype, pages)
+        h = C.c_void_p()
+        check(lib().moe_kv_create(C.byref(h), C.byref(desc)))
+        self.handle = h.value
+
+    @property
+    def pages(self) -> int:
+        return lib().moe_kv_pages(self.handle)
+
+    def append(self, batch, k, v, rope=None, pos=None, q=None, q_out=None, stream=None):
+        check(lib().moe_kv_append(self.handle, C.byref(batch), rope.handle if rope else None, pos,
+                                  _ref(k), _ref(v), _ref(q), _ref(q_out), stream))
+
+    def gather(self, batch, k_out=None, v_out=None, stream=None):
+        check(lib().moe_kv_gather(self.handle, C.byref(batch), _ref(k_out), _ref(v_out), stream))
+
+    def workspace_bytes(self, batch, n_heads) -> int:
+        n = lib().moe_kv_attention_workspace(self.handle, C.byref(batch), n_heads)
+        if n < 0:
+            check(n)
+        return n
+
+    def attention(self, batch, q, out, scale, causal=True, window=0, lse=None, workspace=None,
+                  workspace_bytes=0, stream=None):
+        check(lib().moe_kv_attention(self.handle, C.byref(batch), _ref(q), _ref(out), lse, scale,
+                                     1 if causal else 0, window, workspace, workspace_bytes, stream))
+
+    def status(self) -> int:
+        """waits for the device; the code of moe_kv_status (0 = ok); does not raise"""
+        return lib().moe_kv_status(self.handle)
+
+    def close(self):
+        if getattr(self, "handle", None):
+            lib().moe_kv_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 # ------------------------------------------------------------------ whole model
