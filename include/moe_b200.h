@@ -503,8 +503,7 @@ MOE_API int moe_kv_attention(moe_kv_cache *cache, const moe_kv_batch *batch, con
 			     const moe_rows *out, float *lse, float scale, int causal,
 			     int64_t window, void *workspace, size_t workspace_bytes, void *stream);
 /* Waits for the device; MOE_OK, or (once) MOE_ERR_INVALID if a call since the
- * last one met arrays, pages or positions out of range, MOE_ERR_TIMEOUT if a
- * bounded wait expired. */
+ * last one met arrays, pages or positions out of range. */
 MOE_API int moe_kv_status(moe_kv_cache *cache);
 
 /* ------------------------------------------------------------------ */

@@ -27,12 +27,13 @@
 //
 // Work: an item is a KV head of a sequence, a tile of its query rows (query
 // token x head of the group) and a run of 32-row key tiles; the CTA's 4 warps
-// take the run's tiles in turn, each with a ring of bulk copies of its own, and
-// join their sums at the end.  The run's length is chosen on the device from
+// take the run's tiles in turn, each with a ring of asynchronous copies of its
+// own, and join their sums at the end.  The run's length is chosen on the device from
 // the batch's lengths so that the items fill the GPU however ragged they are;
 // a tile of queries with several runs is joined by a second kernel.
 #include "kv.cuh"
-#include "expert_core.cuh"
+
+#include <type_traits>
 
 namespace moe {
 namespace {
@@ -44,6 +45,7 @@ constexpr int kRunMin = kAttnWarps;          // tiles of a run: one for each war
 constexpr int kRunMax = 256 * kAttnWarps;    // 512 products a warp in one fp32 chain
 constexpr float kLag = 4.0f;       // exponents of 2 that the running maximum may lag
 constexpr float kLift = 10.0f;     // weights are held times 2^10
+constexpr float kNoMax = 3.0e38f;  // the bias kLift - m before any row was seen
 
 struct AttnArgs {
 	BatchArgs b;
@@ -96,113 +98,105 @@ __device__ __forceinline__ int seq_tiles(const AttnArgs &a, int n, int kv)
 	return (kv + kAttnTile - 1) / kAttnTile - lo / kAttnTile;
 }
 
-// sums of v over the CTA's threads before this one, and of all of them
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t &all, int64_t *red)
+__device__ __forceinline__ int64_t warp_sum64(int64_t v)
 {
-	const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-	int64_t s = v;
+#pragma unroll
+	for (int o = 16; o; o /= 2)
+		v += __shfl_xor_sync(0xffffffffu, v, o);
+	return v;
+}
+
+// sums of v over the lanes up to this one
+__device__ __forceinline__ int64_t warp_scan64(int64_t v)
+{
+	const int lane = threadIdx.x % 32;
 #pragma unroll
 	for (int o = 1; o < 32; o *= 2) {
-		const int64_t w = __shfl_up_sync(0xffffffffu, s, o);
-		if (lane >= o)
-			s += w;
+		const int64_t w = __shfl_up_sync(0xffffffffu, v, o);
+		v += lane >= o ? w : 0;
 	}
-	__syncthreads();
-	if (lane == 31)
-		red[warp] = s;
-	__syncthreads();
-	int64_t before = 0;
-	all = 0;
-#pragma unroll
-	for (int w = 0; w < kAttnWarps; w++) {
-		if (w < warp)
-			before += red[w];
-		all += red[w];
-	}
-	return before + s - v;
+	return v;
 }
 
 // Item `index` of the batch (ITEM), or tile `index` of its query tiles with
-// the tile's number of runs.  Every CTA of both kernels derives the same plan
-// from the lengths: all work in key tiles over the items wanted gives the
-// run's length; sums over the sequences before give a sequence's first item.
+// the tile's number of runs.  Every warp of both kernels derives the same plan
+// from the lengths, 32 sequences at a time: all work in key tiles over the
+// items wanted gives the run's length; sums over the sequences before give a
+// sequence's first item.
 template <int RPT, bool ITEM>
-__device__ __forceinline__ bool find_item(const AttnArgs &a, int64_t index, Item &it)
+__device__ __forceinline__ bool find_item(const AttnArgs &a, int64_t index, Item &f)
 {
-	__shared__ int64_t red[kAttnWarps];
-	__shared__ Item found;
-	__shared__ int hit;
-	const int B = a.b.B;
+	const int lane = threadIdx.x % 32, B = a.b.B;
 	int s0 = 0, n = 0, kv = 0;
-	int64_t all = 0;
-	for (int b0 = 0; b0 < B; b0 += kAttnThreads) {
-		const int b = b0 + threadIdx.x;
-		int64_t w = 0, sum;
-		if (b < B && seq_of(a, b, s0, n, kv))
-			w = (int64_t)((n * (int64_t)a.G + RPT - 1) / RPT) * seq_tiles(a, n, kv);
-		block_scan(w, sum, red);
-		all += sum;
-	}
-	all *= a.KVH;
 	int64_t run = (int64_t)1 << 40;   // target 0: query tiles enough, one run each
 	if (a.target) {
-		run = (all + a.target - 1) / a.target;
+		int64_t all = 0;
+		for (int b = lane; b < B; b += 32)
+			if (seq_of(a, b, s0, n, kv))
+				all += (int64_t)((n * a.G + RPT - 1) / RPT) * seq_tiles(a, n, kv);
+		all = warp_sum64(all) * a.KVH;
+		run = (int64_t)ceilf((float)all / a.target);   // about so: any run is right
 		run = run < kRunMin ? kRunMin : run > kRunMax ? kRunMax : run;
 	}
-	if (threadIdx.x == 0)
-		hit = 0;
 	int64_t item0 = 0, tile0 = 0;
-	for (int b0 = 0; b0 < B; b0 += kAttnThreads) {
-		const int b = b0 + threadIdx.x;
-		int64_t tiles = 0, runs = 0, items, sum, tsum;
-		if (B > kAttnThreads) {
+	for (int b0 = 0; b0 < B; b0 += 32) {
+		const int b = b0 + lane;
+		int64_t tiles = 0, runs = 0;
+		if (B > 32 || !a.target) {
 			n = 0;
 			if (b < B)
 				seq_of(a, b, s0, n, kv);
 		}
 		if (b < B && n > 0) {
-			tiles = (n * (int64_t)a.G + RPT - 1) / RPT;
-			runs = (seq_tiles(a, n, kv) + run - 1) / run;
-			runs = runs < 1 ? 1 : runs;
+			const unsigned step = (unsigned)min(run, (int64_t)1 << 30);
+			tiles = (n * a.G + RPT - 1) / RPT;   // the host keeps n G to 2^30
+			runs = max(1u, (seq_tiles(a, n, kv) + step - 1) / step);
 		}
-		items = tiles * runs * a.KVH;
-		const int64_t i0 = item0 + block_scan(items, sum, red);
-		const int64_t q0 = tile0 + block_scan(tiles * a.KVH, tsum, red);
-		const int64_t at = index - (ITEM ? i0 : q0);
-		if (at >= 0 && at < (ITEM ? items : tiles * a.KVH)) {
+		const int64_t items = tiles * runs * a.KVH;
+		const int64_t iend = item0 + warp_scan64(items);
+		const int64_t tend = ITEM ? iend : tile0 + warp_scan64(tiles * a.KVH);
+		const unsigned m = __ballot_sync(0xffffffffu, index < (ITEM ? iend : tend));
+		if (m) {
+			// the first sequence that ends behind it
+			const int src = __ffs(m) - 1;
+			s0 = __shfl_sync(0xffffffffu, s0, src);
+			n = __shfl_sync(0xffffffffu, n, src);
+			kv = __shfl_sync(0xffffffffu, kv, src);
+			tiles = __shfl_sync(0xffffffffu, tiles, src);
+			runs = __shfl_sync(0xffffffffu, runs, src);
+			const int64_t i0 = __shfl_sync(0xffffffffu, iend - items, src);
+			const int64_t t0 = __shfl_sync(0xffffffffu, tend - tiles * a.KVH, src);
+			const int64_t at = index - (ITEM ? i0 : t0);
 			// KV heads side by side; the last tiles, which see the most, first
-			Item f;
-			f.b = b;
+			f.b = b0 + src;
 			f.s0 = s0;
 			f.n = n;
 			f.kv = kv;
-			f.kvh = (int)(at % a.KVH);
-			const int64_t rest = at / a.KVH;
-			f.run = ITEM ? (int)(rest % runs) : 0;
-			const int64_t rank = ITEM ? rest / runs : rest;
-			f.tile = (int)(tiles - 1 - rank);
+			const unsigned rest = (unsigned)at / a.KVH;   // at is below 2^31, as the grid
+			f.kvh = (unsigned)at - rest * a.KVH;
+			const unsigned rank = ITEM ? rest / (unsigned)runs : rest;
+			f.run = ITEM ? rest - rank * (unsigned)runs : 0;
 			const int64_t first = i0 + rank * runs * a.KVH + f.kvh;
 			f.first = (int)first;
+			f.tile = (int)(tiles - 1 - rank);
 			f.r0 = f.tile * RPT;
-			f.rows = (int)min((int64_t)RPT, n * (int64_t)a.G - f.r0);
+			f.rows = min(RPT, n * a.G - f.r0);
 			const int p0 = kv - n + f.r0 / a.G, p1 = kv - n + (f.r0 + f.rows - 1) / a.G;
 			f.lo = a.window ? max(0, p0 - a.window + 1) : 0;
 			f.hi = a.causal ? min(kv, p1 + 1) : kv;
 			const int ta = f.lo / kAttnTile, tb = max(ta, (f.hi + kAttnTile - 1) / kAttnTile);
-			f.runs = max(1, (int)((tb - ta + run - 1) / run));
-			f.t0 = ta + (int)(f.run * run);
+			const unsigned step = (unsigned)min(run, (int64_t)1 << 30);
+			f.runs = max(1u, (tb - ta + step - 1) / step);
+			f.t0 = (int)min((int64_t)tb, ta + f.run * run);
 			f.t1 = (int)min((int64_t)tb, f.t0 + run);
-			found = f;
 			// q_start that does not rise can name more items than it has
 			// tokens for: those behind the plan's bound are left out
-			hit = first + (runs - 1) * a.KVH < a.items;
+			return first + (runs - 1) * a.KVH < a.items && (!ITEM || f.run < f.runs);
 		}
-		item0 += sum;
-		tile0 += tsum;
+		item0 = __shfl_sync(0xffffffffu, iend, 31);
+		tile0 = __shfl_sync(0xffffffffu, tend, 31);
 	}
-	__syncthreads();
-	it = found;
-	return hit && (!ITEM || it.run < it.runs);
+	return false;
 }
 
 __device__ __forceinline__ void mma_step(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -212,6 +206,26 @@ __device__ __forceinline__ void mma_step(float (&d)[4], const uint32_t (&a)[4], 
 		     "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
 		     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
 		     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// the same from a sum of zero
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+					  uint32_t b1)
+{
+	asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+		     "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+		     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+		     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// and from sums of the columns' own
+__device__ __forceinline__ void mma_from(float (&d)[4], float2 c, const uint32_t (&a)[4], uint32_t b0,
+					 uint32_t b1)
+{
+	asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+		     "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+		     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+		     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y));
 }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
@@ -235,18 +249,47 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi)
 	return h2_bits(__floats2half2_rn(lo, hi));
 }
 
-// codes in the low nibbles of bytes 0 and 2 as fp16 code - 8: 1024 + code by
-// placing the nibble in 1024's mantissa, less 1032
+// half `at` of a word
+__device__ __forceinline__ float half_of(uint32_t w, int at)
+{
+	const __half2 h = bits_h2(w);
+	return at ? __high2float(h) : __low2float(h);
+}
+
+__device__ __forceinline__ uint32_t set_half(uint32_t w, int at, float v)
+{
+	const uint32_t h = __half_as_ushort(__float2half_rn(v));
+	return at ? (w & 0xffffu) | h << 16 : (w & 0xffff0000u) | h;
+}
+
+// half `at` of a word, twice
+__device__ __forceinline__ __half2 both(__half2 h, int at)
+{
+	return at ? __high2half2(h) : __low2half2(h);
+}
+
+__device__ __forceinline__ uint32_t smem_addr(const void *p)
+{
+	return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+// Codes as fp16 subnormals: nibbles masked out in place are code * 2^-24 (low
+// nibbles of bytes 0 and 2) and code * 2^-20 (high ones), exact operands of the
+// products for one logic operation a pair.  The -8 of a code: RAW leaves it to
+// the caller, otherwise one exact fp16 subtraction takes it off.
+template <bool RAW>
 __device__ __forceinline__ uint32_t codes_low(uint32_t w)
 {
-	return h2_bits(__hsub2(bits_h2((w & 0x000f000fu) | 0x64006400u), bits_h2(0x64086408u)));
+	const uint32_t x = w & 0x000f000fu;
+	return RAW ? x : h2_bits(__hsub2(bits_h2(x), bits_h2(0x00080008u)));
 }
-// the high nibbles: 1024 + 16 code, over 16, less 72 (each step exact)
+template <bool RAW>
 __device__ __forceinline__ uint32_t codes_high(uint32_t w)
 {
-	return h2_bits(__hfma2(bits_h2((w & 0x00f000f0u) | 0x64006400u), bits_h2(0x2c002c00u),
-			       bits_h2(0xd480d480u)));
+	const uint32_t x = w & 0x00f000f0u;
+	return RAW ? x : h2_bits(__hsub2(bits_h2(x), bits_h2(0x00800080u)));
 }
+constexpr float kCodeUnit = 16777216.0f;   // 2^24
 
 // tile row of A's row j: rows j and j ^ 2.. stay within 16; chosen so that the
 // 8 rows of a shared-memory read touch both halves of the banks
@@ -278,7 +321,7 @@ __device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[NW])
 // with e 0 the row's log-sum-exp
 template <typename T>
 __device__ __forceinline__ void write_row(const AttnArgs &a, const Item &it, int r, int e, float4 v,
-					  float m, float l, bool first)
+					  float b, float l, bool first)
 {
 	const int qr = it.r0 + r, token = it.s0 + qr / a.G, head = it.kvh * a.G + qr % a.G;
 	// nothing seen: zeros
@@ -301,7 +344,7 @@ __device__ __forceinline__ void write_row(const AttnArgs &a, const Item &it, int
 	}
 	if (first && a.lse)
 		a.lse[(int64_t)token * a.H + head] =
-			l == 0.0f ? -__int_as_float(0x7f800000) : 0.693147180559945f * (m + log2f(l) - kLift);
+			l == 0.0f ? -__int_as_float(0x7f800000) : 0.693147180559945f * (log2f(l) - b);
 }
 
 template <int HL>
@@ -320,30 +363,44 @@ constexpr int attn_smem()
 	return ring > join ? ring : join;
 }
 
+#ifndef ATTN_MINB
+#define ATTN_MINB (HL == 128 && NT == 1 ? 4 : 1)
+#endif
 template <int HL, int NT>
 constexpr bool kQInRegs = HL * NT <= 256;
 
+// 16 bytes to shared memory, in flight until its group is waited for
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t *src)
+{
+	asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// all but the newest N groups have landed
+template <int N>
+__device__ __forceinline__ void copies_wait()
+{
+	asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 template <typename T, int HL, int NT>
-__global__ void __launch_bounds__(kAttnThreads) kv_attn_kernel(AttnArgs a)
+__global__ void __launch_bounds__(kAttnThreads, ATTN_MINB) kv_attn_kernel(AttnArgs a)
 {
 	constexpr bool SPLIT = sizeof(T) == 4;        // two columns a row
 	constexpr int RPN = SPLIT ? 4 : 8;            // rows of an 8-column tile
 	constexpr int RPT = RPN * NT, NB = HL / 32, COLS = 8 * NT;
 	constexpr bool QR = kQInRegs<HL, NT>;
+	// one column tile: the keys' -8 sum to -8 sum q, where the scores' sums start
+	constexpr bool KRAW = NT == 1;
 	using SL = StageLayout<HL>;
 	extern __shared__ __align__(128) uint8_t smem[];
-	__shared__ __align__(8) uint64_t bars[kAttnWarps][kAttnStages];
-	__shared__ float sm_m[kAttnWarps][COLS], sm_l[kAttnWarps][COLS];
+	__shared__ float sm_b[kAttnWarps][COLS], sm_l[kAttnWarps][COLS];
 	__shared__ uint2 sm_q[QR ? 1 : 2 * NB * NT][32];
 	__shared__ float sm_qs[COLS];
 	const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
 
 	griddep_launch_dependents();
-	if (threadIdx.x < kAttnWarps * kAttnStages)
-		mbar_init(&bars[0][0] + threadIdx.x, 1);
-	fence_mbar_init();
 	Item it;
-	if (!find_item<RPT, true>(a, blockIdx.x, it))   // its barriers order the inits too
+	if (!find_item<RPT, true>(a, blockIdx.x, it))   // the same for every warp
 		return;
 
 	// ---- the warp's key tiles: t0 + warp, + 4, ..: lane l keeps the pages of
@@ -353,11 +410,9 @@ __global__ void __launch_bounds__(kAttnThreads) kv_attn_kernel(AttnArgs a)
 	const int P = 1 << a.b.page_log2;
 	const bool small = P < kAttnTile;
 	uint8_t *ring = smem + warp * kAttnStages * SL::kBytes;
-	uint64_t *bar = bars[warp];
 	auto key0 = [&](int i) { return (it.t0 + warp + i * kAttnWarps) * kAttnTile; };
 	// which halves of tile i hold rows that the query tile sees
-	auto needs = [&](int i) -> int {
-		const int k0 = key0(i);
+	auto needs = [&](int k0) -> int {
 		return (k0 < it.hi && k0 + 16 > it.lo ? 1 : 0) |
 		       (k0 + 16 < it.hi && k0 + 32 > it.lo ? 2 : 0);
 	};
@@ -365,74 +420,80 @@ __global__ void __launch_bounds__(kAttnThreads) kv_attn_kernel(AttnArgs a)
 	auto load_pages = [&](int i) {
 		page_a = page_b = -1;
 		if (i + lane < ntile) {
-			const int need = needs(i + lane), k0 = key0(i + lane);
-			if (need & (small ? 1 : 3))
+			const int k0 = key0(i + lane), need = needs(k0);
+			const bool wa = need & (small ? 1 : 3), wb = small && (need & 2);
+			if (wa)
 				page_a = table[k0 >> a.b.page_log2];
-			if (small && (need & 2))
+			if (wb)
 				page_b = table[(k0 + 16) >> a.b.page_log2];
-			const bool bad = ((need & (small ? 1 : 3)) && (unsigned)page_a >= (unsigned)a.b.n_pages) ||
-					 (small && (need & 2) && (unsigned)page_b >= (unsigned)a.b.n_pages);
-			if (bad)
+			const bool ba = (unsigned)page_a >= (unsigned)a.b.n_pages;
+			const bool bb = (unsigned)page_b >= (unsigned)a.b.n_pages;
+			if ((wa && ba) || (wb && bb))
 				atomicOr(a.b.err, kKvErrPage);
-			if ((unsigned)page_a >= (unsigned)a.b.n_pages)
-				page_a = -1;
-			if ((unsigned)page_b >= (unsigned)a.b.n_pages)
-				page_b = -1;
+			page_a = ba ? -1 : page_a;
+			page_b = bb ? -1 : page_b;
 		}
 	};
-	// the halves of tile i that are in the ring (pages outside the cache are
-	// not read: their rows count as unseen)
-	auto present = [&](int i) -> int {
-		const int pa = __shfl_sync(0xffffffffu, page_a, i & 31);
-		const int pb = __shfl_sync(0xffffffffu, page_b, i & 31);
-		const int need = needs(i);
-		if (!small)
-			return pa >= 0 ? need : 0;
-		return (pa >= 0 ? need & 1 : 0) | (pb >= 0 ? need & 2 : 0);
-	};
-	const int64_t half_rec = (int64_t)(HL / 2 + HL / 16) << a.b.page_log2;
-	auto copy_rows = [&](uint8_t *st, uint64_t *br, int page, int k0, int at, int n) {
-		const uint8_t *rec = a.pages + page * a.page_bytes + 2 * it.kvh * half_rec;
-		const int r = k0 & (P - 1);
-		const uint8_t *sc = rec + ((int64_t)(HL / 2) << a.b.page_log2);
-		bulk_g2s(st + at * (HL / 2), rec + r * (HL / 2), n * (HL / 2), br);
-		bulk_g2s(st + SL::kKS + at * NB * 2, sc + r * NB * 2, n * NB * 2, br);
-		bulk_g2s(st + SL::kVC + at * (HL / 2), rec + half_rec + r * (HL / 2), n * (HL / 2), br);
-		bulk_g2s(st + SL::kVS + at * NB * 2, sc + half_rec + r * NB * 2, n * NB * 2, br);
-	};
+	const int half_rec = (HL / 2 + HL / 16) << a.b.page_log2;
+	const uint8_t *head_pages = a.pages + 2 * (int64_t)it.kvh * half_rec;
+	// this lane's 16 bytes of every 512 of a tile's codes; of its scales, K's
+	// and V's side by side over the lanes
+	constexpr int CH = SL::kCodes / 512, SLN = SL::kScales / 16, SCH = (2 * SLN + 31) / 32;
+	const uint32_t ring_at = smem_addr(ring) + lane * 16;
 	unsigned ring_have = 0;   // 2 bits a stage: the halves in it
-	auto issue = [&](int i) {
-		const int have = present(i), at = 2 * (i % kAttnStages);
-		ring_have = (ring_have & ~(3u << at)) | (unsigned)have << at;
+	auto issue = [&](int i, int stage) {
+		const int k0 = key0(i);
 		const int pa = __shfl_sync(0xffffffffu, page_a, i & 31);
-		const int pb = __shfl_sync(0xffffffffu, page_b, i & 31);
-		if (lane == 0) {
-			uint8_t *st = ring + (i % kAttnStages) * SL::kBytes;
-			uint64_t *br = bar + i % kAttnStages;
-			const int k0 = key0(i);
-			constexpr int row = 2 * (HL / 2 + NB * 2);
-			mbar_arrive_expect_tx(br, ((have & 1) + (have >> 1)) * 16 * row);
-			if (!small && have == 3) {
-				copy_rows(st, br, pa, k0, 0, 32);
-			} else {
-				if (have & 1)
-					copy_rows(st, br, pa, k0, 0, 16);
-				if (have & 2)
-					copy_rows(st, br, small ? pb : pa, k0 + 16, 16, 16);
+		int pb = pa;
+		if (small)
+			pb = __shfl_sync(0xffffffffu, page_b, i & 31);
+		// pages outside the cache are not read: their rows count as unseen
+		const int have = needs(k0) & ((pa >= 0 ? 1 : 0) | (pb >= 0 ? 2 : 0));
+		ring_have = (ring_have & ~(3u << 2 * stage)) | (unsigned)have << 2 * stage;
+		const uint32_t st = ring_at + stage * SL::kBytes;
+		const int r = k0 & (P - 1);
+		const uint8_t *src = head_pages + pa * a.page_bytes + r * (HL / 2) + lane * 16;
+		// the second half's rows: 16 further on, or another page's first
+		const uint8_t *src2 = small ? head_pages + pb * a.page_bytes + lane * 16 - 16 * (HL / 2) : src;
+#pragma unroll
+		for (int q = 0; q < CH; q++) {
+			const uint8_t *p = (q < CH / 2 ? src : src2) + 512 * q;
+			if (have >> (q < CH / 2 ? 0 : 1) & 1) {
+				copy16(st + 512 * q, p);
+				copy16(st + SL::kVC + 512 * q, p + half_rec);
+			}
+		}
+#pragma unroll
+		for (int q = 0; q < SCH; q++) {
+			const int j = lane + 32 * q, isv = j >= SLN, jj = isv ? j - SLN : j;
+			const int h = jj * 2 >= SLN;
+			if (j < 2 * SLN && (have >> h & 1)) {
+				const int row = small && h ? -16 : r;
+				const uint8_t *p = head_pages + (small && h ? pb : pa) * a.page_bytes +
+						   (((HL / 2) << a.b.page_log2) + (isv ? half_rec : 0) +
+						    row * NB * 2 + jj * 16);
+				copy16(st - lane * 16 + (isv ? SL::kVS : SL::kKS) + jj * 16, p);
 			}
 		}
 	};
 	load_pages(0);
-	const int pre = min(ntile, kAttnStages);
-	for (int i = 0; i < pre; i++)
-		issue(i);
+#pragma unroll
+	for (int i = 0; i < kAttnStages - 1; i++) {
+		if (i < ntile)
+			issue(i, i);
+		copies_commit();
+	}
 
 	// ---- the queries: column n = g of every 8-column tile, values 4 c .. of
 	// each half block, as B fragments
 	uint2 qf[QR ? 2 * NB * NT : 1];
+	float2 q_off[KRAW ? NB : 1];
 	const T *qp = static_cast<const T *>(a.q) + (int64_t)it.kvh * a.G * a.q_hs;
 	float qs_own[QR ? NT : 1];
-	for (int nt = QR ? 0 : warp; nt < NT; nt += QR ? 1 : kAttnWarps) {
+#pragma unroll
+	for (int nt = 0; nt < NT; nt++) {
+		if (!QR && nt % kAttnWarps != warp)
+			continue;   // one warp each, through shared memory
 		const int r = nt * RPN + (SPLIT ? g / 2 : g);
 		float x[HL / 4];
 		if (r < it.rows) {
@@ -463,32 +524,46 @@ __global__ void __launch_bounds__(kAttnThreads) kv_attn_kernel(AttnArgs a)
 			for (int k = 0; k < HL / 4; k++)
 				x[k] = 0.0f;
 		}
-		float top = 0.0f;
-		bool bad = false;
+		// the largest magnitude, by its bits: an infinity or a NaN is above all
+		uint32_t bits = 0;
 #pragma unroll
-		for (int k = 0; k < HL / 4; k++) {
-			top = fmaxf(top, fabsf(x[k]));
-			bad |= !(fabsf(x[k]) <= 3.402823466e38f);
-		}
-		top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-		top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-		const unsigned badm = __ballot_sync(0xffffffffu, bad);
-		bad = (badm >> (4 * g)) & 15;
+		for (int k = 0; k < HL / 4; k++)
+			bits = max(bits, __float_as_uint(x[k]) & 0x7fffffffu);
+		bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
+		bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
+		const float top = __uint_as_float(bits);
+		const bool bad = bits >= 0x7f800000u;
 		const int e = top > 0.0f && !bad ? 13 - ilogbf(top) : 0;   // -114 .. 162
 		const float up0 = __int_as_float((127 + e / 2) << 23);
 		const float up1 = __int_as_float((127 + e - e / 2) << 23);
 		// a query with an infinity or a NaN has no finite scores: NaN
-		const float qs = bad ? __int_as_float(0x7fffffff) : scalbnf(a.scale2, -e);
+		const float qs = bad ? __int_as_float(0x7fffffff) : scalbnf(a.scale2 * kCodeUnit, -e);
 #pragma unroll
 		for (int k = 0; k < HL / 4; k++) {
 			const float v = bad ? 0.0f : x[k] * up0 * up1;
 			const float hi = __half2float(__float2half_rn(v));
 			x[k] = SPLIT && (g & 1) ? v - hi : hi;
 		}
+		if constexpr (KRAW) {
+			// -8 sum of the column's values of each block, as rounded
+#pragma unroll
+			for (int b = 0; b < NB; b++) {
+				float t = 0.0f;
+#pragma unroll
+				for (int k = 0; k < 8; k++)
+					t += __half2float(__float2half_rn(x[8 * b + k]));
+				t += __shfl_xor_sync(0xffffffffu, t, 1);
+				t += __shfl_xor_sync(0xffffffffu, t, 2);
+				t *= -8.0f / kCodeUnit;
+				q_off[b] = make_float2(__shfl_sync(0xffffffffu, t, 8 * c),
+						       __shfl_sync(0xffffffffu, t, 8 * c + 4));
+			}
+		}
 #pragma unroll
 		for (int h = 0; h < HL / 16; h++) {
-			const uint2 f = make_uint2(pack_h2(x[4 * h], x[4 * h + 2]),
-						   pack_h2(x[4 * h + 1], x[4 * h + 3]));
+			const float u = h & 1 ? 0.0625f : 1.0f;   // high nibbles count 16-fold
+			const uint2 f = make_uint2(pack_h2(x[4 * h] * u, x[4 * h + 2] * u),
+						   pack_h2(x[4 * h + 1] * u, x[4 * h + 3] * u));
 			if constexpr (QR)
 				qf[nt * 2 * NB + h] = f;
 			else
@@ -514,18 +589,15 @@ __global__ void __launch_bounds__(kAttnThreads) kv_attn_kernel(AttnArgs a)
 		}
 	}
 	// the cache row at which each column's query stands
-	int row0[NT], row1[NT];
-#pragma unroll
-	for (int nt = 0; nt < NT; nt++) {
-		const int ra = it.r0 + nt * RPN + (SPLIT ? c : 2 * c);
-		row0[nt] = it.kv - it.n + ra / a.G;
-		row1[nt] = SPLIT ? row0[nt] : it.kv - it.n + (ra + 1) / a.G;
-	}
-	const int first_row = it.kv - it.n + it.r0 / a.G;
-	const int last_row = it.kv - it.n + (it.r0 + it.rows - 1) / a.G;
+	auto row_of = [&](int r) { return it.kv - it.n + (it.r0 + r) / a.G; };
+	auto row0 = [&](int nt) { return row_of(nt * RPN + (SPLIT ? c : 2 * c)); };
+	auto row1 = [&](int nt) { return row_of(nt * RPN + (SPLIT ? c : 2 * c + 1)); };
+	const int first_row = row_of(0), last_row = row_of(it.rows - 1);
 
+	// running sums of columns 2 c (0) and 2 c + 1 (1): o and l relative to the
+	// largest score m so far, kept as b = kLift - m
 	float o[2 * NB][NT][4];
-	float m0[NT], m1[NT], l0[NT], l1[NT], rv[NB];
+	float b0[NT], b1[NT], l0[NT], l1[NT];
 #pragma unroll
 	for (int i = 0; i < 2 * NB; i++)
 #pragma unroll
@@ -535,109 +607,264 @@ __global__ void __launch_bounds__(kAttnThreads) kv_attn_kernel(AttnArgs a)
 				o[i][nt][k] = 0.0f;
 #pragma unroll
 	for (int nt = 0; nt < NT; nt++) {
-		m0[nt] = m1[nt] = -3.0e38f;
+		b0[nt] = b1[nt] = kNoMax;
 		l0[nt] = l1[nt] = 0.0f;
 	}
+	// the V scales' factors, a power of two for each block, two to a word, and
+	// the largest scales that they hold in range (2 over the factor)
+	uint32_t v_fac[NB / 2], v_top[NB / 2];
 #pragma unroll
-	for (int b = 0; b < NB; b++)
-		rv[b] = 1.7014118e38f;   // 2^127: the first V scale sets it
+	for (int k = 0; k < NB / 2; k++) {
+		v_fac[k] = 0x78007800u;   // 2^15
+		v_top[k] = 0x04000400u;   // 2^-14
+	}
+	// scores up to a0, a1 (in exponents of 2) seen
+	auto raise = [&](int nt, float a0, float a1) {
+		const float n0 = fminf(b0[nt], kLift - a0), n1 = fminf(b1[nt], kLift - a1);
+		const float f0 = ex2(n0 - b0[nt]), f1 = ex2(n1 - b1[nt]);
+		b0[nt] = n0;
+		b1[nt] = n1;
+		l0[nt] *= f0;
+		l1[nt] *= f1;
+#pragma unroll
+		for (int k = 0; k < 2 * NB; k++) {
+			o[k][nt][0] *= f0;
+			o[k][nt][1] *= f1;
+			o[k][nt][2] *= f0;
+			o[k][nt][3] *= f1;
+		}
+	};
 
 	const int ja = tile_row(g);                                  // A's rows g and g + 8
 	const int va = tile_row(2 * c), vb = tile_row(2 * c + 1);    // A's columns 2 c ..
-	int i = 0;
-	for (; i < ntile; i++) {
-		if (!mbar_wait(bar + i % kAttnStages, (i / kAttnStages) & 1))
-			break;
-		const uint8_t *st = ring + (i % kAttnStages) * SL::kBytes;
-		const int have = ring_have >> (2 * (i % kAttnStages)) & 3;
-		const int k0 = key0(i);
-		const bool full = have == 3 && k0 >= it.lo && k0 + kAttnTile <= it.kv &&
-				  (!a.causal || k0 + kAttnTile - 1 <= first_row) &&
-				  (!a.window || k0 > last_row - a.window);
-#pragma unroll 1
-		for (int u = 0; u < 2; u++) {
-			if (!(have >> u & 1))
-				continue;
-			const int base = 16 * u;
-			// ---- scores
-			float s[NT][4];
+	// 16 rows of a tile (FULL: every query of the item sees them all)
+	auto rows16 = [&](auto full_c, const uint8_t *st, int base, int k0) {
+		constexpr bool FULL = decltype(full_c)::value;
+		// ---- scores
+		float s[NT][4];
 #pragma unroll
-			for (int nt = 0; nt < NT; nt++)
+		for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+			for (int k = 0; k < 4; k++)
+				s[nt][k] = 0.0f;
+		{
+			uint32_t ka[NB], kb[NB], da[NB / 2], db[NB / 2];
+			const uint8_t *kp = st + (base + ja) * (HL / 2) + c * 4 * NB;
+			lds_words<NB>(kp, ka);
+			lds_words<NB>(kp + 8 * (HL / 2), kb);
+			const uint8_t *ks = st + SL::kKS + (base + ja) * NB * 2;
+			lds_words<NB / 2>(ks, da);
+			lds_words<NB / 2>(ks + 8 * NB * 2, db);
+#pragma unroll
+			for (int b = 0; b < NB; b++) {
+				const uint32_t lo[4] = {codes_low<KRAW>(ka[b]), codes_low<KRAW>(kb[b]),
+							codes_low<KRAW>(ka[b] >> 8), codes_low<KRAW>(kb[b] >> 8)};
+				const uint32_t hi[4] = {codes_high<KRAW>(ka[b]), codes_high<KRAW>(kb[b]),
+							codes_high<KRAW>(ka[b] >> 8),
+							codes_high<KRAW>(kb[b] >> 8)};
+				const float dka = half_of(da[b / 2], b & 1), dkb = half_of(db[b / 2], b & 1);
+#pragma unroll
+				for (int nt = 0; nt < NT; nt++) {
+					uint2 q0, q1;
+					if constexpr (QR) {
+						q0 = qf[nt * 2 * NB + 2 * b];
+						q1 = qf[nt * 2 * NB + 2 * b + 1];
+					} else {
+						q0 = sm_q[nt * 2 * NB + 2 * b][lane];
+						q1 = sm_q[nt * 2 * NB + 2 * b + 1][lane];
+					}
+					float d[4];
+					if constexpr (KRAW)
+						mma_from(d, q_off[b], lo, q0.x, q0.y);
+					else
+						mma_first(d, lo, q0.x, q0.y);
+					mma_step(d, hi, q1.x, q1.y);
+					s[nt][0] = fmaf(dka, d[0], s[nt][0]);
+					s[nt][1] = fmaf(dka, d[1], s[nt][1]);
+					s[nt][2] = fmaf(dkb, d[2], s[nt][2]);
+					s[nt][3] = fmaf(dkb, d[3], s[nt][3]);
+				}
+			}
+		}
+		// ---- weights, times 2^kLift over the largest so far
+		const int kra = k0 + base + ja, krb = kra + 8;
+		float p[NT][4];
+		bool seen[NT][4], lag = false;
+#pragma unroll
+		for (int nt = 0; nt < NT; nt++) {
+			if (SPLIT) {
+				s[nt][0] += s[nt][1];
+				s[nt][2] += s[nt][3];
+			}
+			p[nt][0] = fmaf(s[nt][0], qs0[nt], b0[nt]);
+			p[nt][2] = fmaf(s[nt][2], qs0[nt], b0[nt]);
+			p[nt][1] = SPLIT ? p[nt][0] : fmaf(s[nt][1], qs1[nt], b1[nt]);
+			p[nt][3] = SPLIT ? p[nt][2] : fmaf(s[nt][3], qs1[nt], b1[nt]);
+			if (!FULL) {
+				auto sees = [&](int j, int row) {
+					return j < it.kv && (!a.causal || j <= row) &&
+					       (!a.window || j > row - a.window);
+				};
+				seen[nt][0] = sees(kra, row0(nt));
+				seen[nt][2] = sees(krb, row0(nt));
+				seen[nt][1] = SPLIT ? seen[nt][0] : sees(kra, row1(nt));
+				seen[nt][3] = SPLIT ? seen[nt][2] : sees(krb, row1(nt));
+			}
+#pragma unroll
+			for (int k = 0; k < 4; k += SPLIT ? 2 : 1)
+				lag |= (FULL || seen[nt][k]) && p[nt][k] > kLift + kLag;
+		}
+		if (__any_sync(0xffffffffu, lag)) {
+#pragma unroll
+			for (int nt = 0; nt < NT; nt++) {
+				float t[4];
+#pragma unroll
+				for (int k = 0; k < 4; k++) {
+					const bool first = SPLIT || k % 2 == 0;
+					t[k] = s[nt][SPLIT ? k & 2 : k] * (first ? qs0[nt] : qs1[nt]);
+					if (!FULL)
+						t[k] = seen[nt][k] ? t[k] : -kNoMax;
+				}
+				float a0 = fmaxf(t[0], t[2]), a1 = fmaxf(t[1], t[3]);
+#pragma unroll
+				for (int x = 4; x < 32; x *= 2) {
+					a0 = fmaxf(a0, __shfl_xor_sync(0xffffffffu, a0, x));
+					a1 = fmaxf(a1, __shfl_xor_sync(0xffffffffu, a1, x));
+				}
+				raise(nt, a0, a1);
+				p[nt][0] = fmaf(s[nt][0], qs0[nt], b0[nt]);
+				p[nt][2] = fmaf(s[nt][2], qs0[nt], b0[nt]);
+				p[nt][1] = SPLIT ? p[nt][0] : fmaf(s[nt][1], qs1[nt], b1[nt]);
+				p[nt][3] = SPLIT ? p[nt][2] : fmaf(s[nt][3], qs1[nt], b1[nt]);
+			}
+		}
+#pragma unroll
+		for (int nt = 0; nt < NT; nt++) {
+			p[nt][0] = ex2(p[nt][0]);
+			p[nt][2] = ex2(p[nt][2]);
+			p[nt][1] = SPLIT ? p[nt][0] : ex2(p[nt][1]);
+			p[nt][3] = SPLIT ? p[nt][2] : ex2(p[nt][3]);
+			if (!FULL) {
 #pragma unroll
 				for (int k = 0; k < 4; k++)
-					s[nt][k] = 0.0f;
-			{
-				uint32_t ka[NB], kb[NB], da[NB / 2], db[NB / 2];
-				const uint8_t *kp = st + (base + ja) * (HL / 2) + c * 4 * NB;
-				lds_words<NB>(kp, ka);
-				lds_words<NB>(kp + 8 * (HL / 2), kb);
-				const uint8_t *ks = st + SL::kKS + (base + ja) * NB * 2;
-				lds_words<NB / 2>(ks, da);
-				lds_words<NB / 2>(ks + 8 * NB * 2, db);
+					p[nt][k] = seen[nt][k] ? p[nt][k] : 0.0f;
+			}
+			l0[nt] += p[nt][0] + p[nt][2];
+			if (!SPLIT)
+				l1[nt] += p[nt][1] + p[nt][3];
+		}
+		// ---- O += V^T P^T
+		uint32_t wa[NB / 2], wb[NB / 2];
+		const uint8_t *vs = st + SL::kVS + (base + ja) * NB * 2;
+		lds_words<NB / 2>(vs, wa);
+		lds_words<NB / 2>(vs + 8 * NB * 2, wb);
 #pragma unroll
-				for (int b = 0; b < NB; b++) {
-					const uint32_t lo[4] = {codes_low(ka[b]), codes_low(kb[b]),
-								codes_low(ka[b] >> 8), codes_low(kb[b] >> 8)};
-					const uint32_t hi[4] = {codes_high(ka[b]), codes_high(kb[b]),
-								codes_high(ka[b] >> 8), codes_high(kb[b] >> 8)};
-					const float dka = half_bits_to_float((uint16_t)(da[b / 2] >> (16 * (b & 1))));
-					const float dkb = half_bits_to_float((uint16_t)(db[b / 2] >> (16 * (b & 1))));
+		for (int k = 0; k < NB / 2; k++) {
+			wa[k] = h2_bits(__hmul2(bits_h2(wa[k]), bits_h2(v_fac[k])));
+			wb[k] = h2_bits(__hmul2(bits_h2(wb[k]), bits_h2(v_fac[k])));
+		}
+		uint32_t p2[NT][2], keep[NT][2];   // 16-bit rows: two columns' weights, and what of them is seen
 #pragma unroll
-					for (int nt = 0; nt < NT; nt++) {
-						uint2 q0, q1;
-						if constexpr (QR) {
-							q0 = qf[nt * 2 * NB + 2 * b];
-							q1 = qf[nt * 2 * NB + 2 * b + 1];
-						} else {
-							q0 = sm_q[nt * 2 * NB + 2 * b][lane];
-							q1 = sm_q[nt * 2 * NB + 2 * b + 1][lane];
-						}
-						float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-						mma_step(d, lo, q0.x, q0.y);
-						mma_step(d, hi, q1.x, q1.y);
-						s[nt][0] = fmaf(dka, d[0], s[nt][0]);
-						s[nt][1] = fmaf(dka, d[1], s[nt][1]);
-						s[nt][2] = fmaf(dkb, d[2], s[nt][2]);
-						s[nt][3] = fmaf(dkb, d[3], s[nt][3]);
+		for (int nt = 0; nt < NT; nt++) {
+			if (SPLIT)
+				continue;
+			p2[nt][0] = pack_h2(p[nt][0], p[nt][1]);
+			p2[nt][1] = pack_h2(p[nt][2], p[nt][3]);
+			if (!FULL) {
+				keep[nt][0] = (seen[nt][0] ? 0xffffu : 0) | (seen[nt][1] ? 0xffff0000u : 0);
+				keep[nt][1] = (seen[nt][2] ? 0xffffu : 0) | (seen[nt][3] ? 0xffff0000u : 0);
+			}
+		}
+		uint32_t v0[NB / 2], v1[NB / 2], v2[NB / 2], v3[NB / 2];
+		const uint8_t *vp = st + SL::kVC + base * (HL / 2) + g * 2 * NB;
+		lds_words<NB / 2>(vp + va * (HL / 2), v0);
+		lds_words<NB / 2>(vp + vb * (HL / 2), v1);
+		lds_words<NB / 2>(vp + (va + 8) * (HL / 2), v2);
+		lds_words<NB / 2>(vp + (vb + 8) * (HL / 2), v3);
+#pragma unroll
+		for (int b = 0; b < NB; b++) {
+			// bytes 2 g, 2 g + 1 of the block, of two rows each
+			const uint32_t sel0 = b & 1 ? 0x0602 : 0x0400, sel1 = b & 1 ? 0x0703 : 0x0501;
+			const uint32_t t0 = __byte_perm(v0[b / 2], v1[b / 2], sel0);
+			const uint32_t t1 = __byte_perm(v0[b / 2], v1[b / 2], sel1);
+			const uint32_t t2 = __byte_perm(v2[b / 2], v3[b / 2], sel0);
+			const uint32_t t3 = __byte_perm(v2[b / 2], v3[b / 2], sel1);
+			const uint32_t lo[4] = {codes_low<false>(t0), codes_low<false>(t1), codes_low<false>(t2),
+						codes_low<false>(t3)};
+			const uint32_t hi[4] = {codes_high<false>(t0), codes_high<false>(t1),
+						codes_high<false>(t2), codes_high<false>(t3)};
+			// the rows' weights of this block
+			const __half2 da = both(bits_h2(wa[b / 2]), b & 1), db = both(bits_h2(wb[b / 2]), b & 1);
+#pragma unroll
+			for (int nt = 0; nt < NT; nt++) {
+				uint32_t x0, x1;
+				if (SPLIT) {
+					float w0 = p[nt][0] * __low2float(da), w1 = p[nt][2] * __low2float(db);
+					if (!FULL) {   // a row unseen may hold a NaN scale
+						w0 = seen[nt][0] ? w0 : 0.0f;
+						w1 = seen[nt][2] ? w1 : 0.0f;
+					}
+					const float h0 = __half2float(__float2half_rn(w0));
+					const float h1 = __half2float(__float2half_rn(w1));
+					x0 = pack_h2(h0, w0 - h0);
+					x1 = pack_h2(h1, w1 - h1);
+				} else {
+					x0 = h2_bits(__hmul2(bits_h2(p2[nt][0]), da));
+					x1 = h2_bits(__hmul2(bits_h2(p2[nt][1]), db));
+					if (!FULL) {
+						x0 &= keep[nt][0];
+						x1 &= keep[nt][1];
 					}
 				}
+				x0 = transpose8x8(x0);
+				x1 = transpose8x8(x1);
+				mma_step(o[2 * b][nt], lo, x0, x1);
+				mma_step(o[2 * b + 1][nt], hi, x0, x1);
 			}
-			// ---- V scales of this lane's two rows
-			const int kra = k0 + base + ja, krb = kra + 8;
-			float dva[NB], dvb[NB];
-			{
-				uint32_t wa[NB / 2], wb[NB / 2];
-				const uint8_t *vs = st + SL::kVS + (base + ja) * NB * 2;
-				lds_words<NB / 2>(vs, wa);
-				lds_words<NB / 2>(vs + 8 * NB * 2, wb);
-				if (!full) {
-					// rows that no query of the tile sees hold anything
-#pragma unroll
-					for (int k = 0; k < NB / 2; k++) {
-						wa[k] = kra < it.hi && kra >= it.lo ? wa[k] : 0;
-						wb[k] = krb < it.hi && krb >= it.lo ? wb[k] : 0;
-					}
-				}
-#pragma unroll
-				for (int b = 0; b < NB; b++) {
-					dva[b] = half_bits_to_float((uint16_t)(wa[b / 2] >> (16 * (b & 1))));
-					dvb[b] = half_bits_to_float((uint16_t)(wb[b / 2] >> (16 * (b & 1))));
-				}
-			}
+		}
+	};
+
+	// rows that every query of the item sees
+	const int all_lo = a.window ? max(it.lo, last_row - a.window + 1) : it.lo;
+	const int all_hi = a.causal ? min(it.kv, first_row + 1) : it.kv;
+	int stage = 0;
+	for (int i = 0; i < ntile; i++) {
+		copies_wait<kAttnStages - 2>();
+		__syncwarp();   // every lane's copies are in, and the stage before is read
+		{
+			const int next = i + kAttnStages - 1;
+			if ((next & 31) == 0)
+				load_pages(next);
+			if (next < ntile)
+				issue(next, stage == 0 ? kAttnStages - 1 : stage - 1);
+			copies_commit();
+		}
+		const uint8_t *st = ring + stage * SL::kBytes;
+		const int have = ring_have >> (2 * stage) & 3;
+		const int k0 = key0(i);
+		const bool full = have == 3 && k0 >= all_lo && k0 + kAttnTile <= all_hi;
+		// ---- the V scales' range: lane = row (rows not in the ring, or that
+		// no query sees, may hold anything)
+		{
+			uint32_t w[NB / 2];
+			lds_words<NB / 2>(st + SL::kVS + lane * NB * 2, w);
+			const bool use = full || ((have >> (lane / 16) & 1) && k0 + lane >= it.lo &&
+						  k0 + lane < it.hi);
 			bool grow = false;
 #pragma unroll
-			for (int b = 0; b < NB; b++)
-				grow |= fmaxf(fabsf(dva[b]), fabsf(dvb[b])) * rv[b] > 2.0f;
-			if (__any_sync(0xffffffffu, grow)) {
-				// the largest V scale so far to [1, 2): a power of two
+			for (int k = 0; k < NB / 2; k++)
+				grow |= !__hble2(__habs2(bits_h2(w[k])), bits_h2(v_top[k]));
+			if (__any_sync(0xffffffffu, grow && use)) {
+				// the largest so far to [1, 2): a power of two from 2^15 down
 #pragma unroll
 				for (int b = 0; b < NB; b++) {
-					float v = fmaxf(fabsf(dva[b]), fabsf(dvb[b]));
-					v = warp_max(v);
-					if (v * rv[b] > 2.0f) {
-						const float r = scalbnf(1.0f, -ilogbf(v));
-						const float f = r / rv[b];
-						rv[b] = r;
+					const float v = warp_max(use ? fabsf(half_of(w[b / 2], b & 1)) : 0.0f);
+					const float had = half_of(v_fac[b / 2], b & 1);
+					if (v * had > 2.0f) {
+						const float r = scalbnf(1.0f, -min(ilogbf(v), 15));
+						const float f = r / had;
+						v_fac[b / 2] = set_half(v_fac[b / 2], b & 1, r);
+						v_top[b / 2] = set_half(v_top[b / 2], b & 1, 2.0f / r);
 #pragma unroll
 						for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -648,150 +875,20 @@ __global__ void __launch_bounds__(kAttnThreads) kv_attn_kernel(AttnArgs a)
 					}
 				}
 			}
-#pragma unroll
-			for (int b = 0; b < NB; b++) {
-				dva[b] *= rv[b];
-				dvb[b] *= rv[b];
-			}
-			// ---- weights
-			float p[NT][4];
-			bool seen[NT][4];
-			bool lag = false;
-#pragma unroll
-			for (int nt = 0; nt < NT; nt++) {
-				if (SPLIT) {
-					s[nt][0] = (s[nt][0] + s[nt][1]) * qs0[nt];
-					s[nt][2] = (s[nt][2] + s[nt][3]) * qs0[nt];
-					s[nt][1] = s[nt][0];
-					s[nt][3] = s[nt][2];
-				} else {
-					s[nt][0] *= qs0[nt];
-					s[nt][1] *= qs1[nt];
-					s[nt][2] *= qs0[nt];
-					s[nt][3] *= qs1[nt];
-				}
-#pragma unroll
-				for (int k = 0; k < 4; k++)
-					seen[nt][k] = true;
-				if (!full) {
-					auto sees = [&](int j, int row) {
-						return j < it.kv && (!a.causal || j <= row) &&
-						       (!a.window || j > row - a.window);
-					};
-					seen[nt][0] = sees(kra, row0[nt]);
-					seen[nt][2] = sees(krb, row0[nt]);
-					seen[nt][1] = SPLIT ? seen[nt][0] : sees(kra, row1[nt]);
-					seen[nt][3] = SPLIT ? seen[nt][2] : sees(krb, row1[nt]);
-				}
-				lag |= (seen[nt][0] && s[nt][0] > m0[nt] + kLag) ||
-				       (seen[nt][2] && s[nt][2] > m0[nt] + kLag);
-				if (!SPLIT)
-					lag |= (seen[nt][1] && s[nt][1] > m1[nt] + kLag) ||
-					       (seen[nt][3] && s[nt][3] > m1[nt] + kLag);
-			}
-			if (__any_sync(0xffffffffu, lag)) {
-#pragma unroll
-				for (int nt = 0; nt < NT; nt++) {
-					float a0 = fmaxf(seen[nt][0] ? s[nt][0] : -3.0e38f,
-							 seen[nt][2] ? s[nt][2] : -3.0e38f);
-					float a1 = fmaxf(seen[nt][1] ? s[nt][1] : -3.0e38f,
-							 seen[nt][3] ? s[nt][3] : -3.0e38f);
-#pragma unroll
-					for (int x = 4; x < 32; x *= 2) {
-						a0 = fmaxf(a0, __shfl_xor_sync(0xffffffffu, a0, x));
-						a1 = fmaxf(a1, __shfl_xor_sync(0xffffffffu, a1, x));
-					}
-					a0 = fmaxf(a0, m0[nt]);
-					a1 = fmaxf(a1, m1[nt]);
-					const float f0 = ex2(m0[nt] - a0), f1 = ex2(m1[nt] - a1);
-					m0[nt] = a0;
-					m1[nt] = a1;
-					l0[nt] *= f0;
-					l1[nt] *= f1;
-#pragma unroll
-					for (int k = 0; k < 2 * NB; k++) {
-						o[k][nt][0] *= f0;
-						o[k][nt][1] *= f1;
-						o[k][nt][2] *= f0;
-						o[k][nt][3] *= f1;
-					}
-				}
-			}
-#pragma unroll
-			for (int nt = 0; nt < NT; nt++) {
-				const float b0 = kLift - m0[nt], b1 = kLift - m1[nt];
-				p[nt][0] = ex2(s[nt][0] + b0);
-				p[nt][2] = ex2(s[nt][2] + b0);
-				p[nt][1] = SPLIT ? p[nt][0] : ex2(s[nt][1] + b1);
-				p[nt][3] = SPLIT ? p[nt][2] : ex2(s[nt][3] + b1);
-				if (!full) {
-#pragma unroll
-					for (int k = 0; k < 4; k++)
-						p[nt][k] = seen[nt][k] ? p[nt][k] : 0.0f;
-				}
-				l0[nt] += p[nt][0] + p[nt][2];
-				l1[nt] += p[nt][1] + p[nt][3];
-			}
-			// ---- O += V^T P^T
-			uint32_t v0[NB / 2], v1[NB / 2], v2[NB / 2], v3[NB / 2];
-			const uint8_t *vp = st + SL::kVC + base * (HL / 2) + g * 2 * NB;
-			lds_words<NB / 2>(vp + va * (HL / 2), v0);
-			lds_words<NB / 2>(vp + vb * (HL / 2), v1);
-			lds_words<NB / 2>(vp + (va + 8) * (HL / 2), v2);
-			lds_words<NB / 2>(vp + (vb + 8) * (HL / 2), v3);
-#pragma unroll
-			for (int b = 0; b < NB; b++) {
-				// bytes 2 g, 2 g + 1 of the block, of two rows each
-				const uint32_t sel0 = b & 1 ? 0x0602 : 0x0400;
-				const uint32_t sel1 = b & 1 ? 0x0703 : 0x0501;
-				const uint32_t t0 = __byte_perm(v0[b / 2], v1[b / 2], sel0);
-				const uint32_t t1 = __byte_perm(v0[b / 2], v1[b / 2], sel1);
-				const uint32_t t2 = __byte_perm(v2[b / 2], v3[b / 2], sel0);
-				const uint32_t t3 = __byte_perm(v2[b / 2], v3[b / 2], sel1);
-				const uint32_t lo[4] = {codes_low(t0), codes_low(t1), codes_low(t2), codes_low(t3)};
-				const uint32_t hi[4] = {codes_high(t0), codes_high(t1), codes_high(t2),
-							codes_high(t3)};
-#pragma unroll
-				for (int nt = 0; nt < NT; nt++) {
-					float w[4];
-#pragma unroll
-					for (int k = 0; k < 4; k++) {
-						w[k] = p[nt][k] * (k < 2 ? dva[b] : dvb[b]);
-						if (!full)   // a row unseen may hold a NaN scale
-							w[k] = seen[nt][k] ? w[k] : 0.0f;
-					}
-					uint32_t b0, b1;
-					if (SPLIT) {
-						const float h0 = __half2float(__float2half_rn(w[0]));
-						const float h1 = __half2float(__float2half_rn(w[2]));
-						b0 = pack_h2(h0, w[0] - h0);
-						b1 = pack_h2(h1, w[2] - h1);
-					} else {
-						b0 = pack_h2(w[0], w[1]);
-						b1 = pack_h2(w[2], w[3]);
-					}
-					b0 = transpose8x8(b0);
-					b1 = transpose8x8(b1);
-					mma_step(o[2 * b][nt], lo, b0, b1);
-					mma_step(o[2 * b + 1][nt], hi, b0, b1);
-				}
-			}
 		}
-		__syncwarp();   // every lane has read the stage
-		const int next = i + kAttnStages;
-		if ((next & 31) == 0 && next < ntile)
-			load_pages(next);
-		if (next < ntile)
-			issue(next);
+		if (full) {
+#pragma unroll 1
+			for (int u = 0; u < 2; u++)
+				rows16(std::true_type{}, st, 16 * u, k0);
+		} else {
+#pragma unroll 1
+			for (int u = 0; u < 2; u++)
+				if (have >> u & 1)
+					rows16(std::false_type{}, st, 16 * u, k0);
+		}
+		stage = stage + 1 == kAttnStages ? 0 : stage + 1;
 	}
-	if (i < ntile) {
-		// a wait ran out: the copies still in flight (each waited for once
-		// more) must not land in memory that is used below
-		if (lane == 0)
-			atomicOr(a.b.err, kKvErrWait);
-		for (int s = i; s < min(ntile, i + kAttnStages); s++)
-			mbar_wait(bar + s % kAttnStages, (s / kAttnStages) & 1);
-	}
+	copies_wait<0>();
 
 	// ---- the warps' sums joined, over the ring's memory
 #pragma unroll
@@ -801,31 +898,33 @@ __global__ void __launch_bounds__(kAttnThreads) kv_attn_kernel(AttnArgs a)
 			l0[nt] += __shfl_xor_sync(0xffffffffu, l0[nt], x);
 			l1[nt] += __shfl_xor_sync(0xffffffffu, l1[nt], x);
 		}
+		if (SPLIT)
+			l1[nt] = l0[nt];
 		if (g == 0) {
-			sm_m[warp][nt * 8 + 2 * c] = m0[nt];
-			sm_m[warp][nt * 8 + 2 * c + 1] = m1[nt];
+			sm_b[warp][nt * 8 + 2 * c] = b0[nt];
+			sm_b[warp][nt * 8 + 2 * c + 1] = b1[nt];
 			sm_l[warp][nt * 8 + 2 * c] = l0[nt];
 			sm_l[warp][nt * 8 + 2 * c + 1] = l1[nt];
 		}
 	}
 	__syncthreads();
-	auto top_of = [&](int col) {
-		float m = sm_m[0][col];
+	auto bias_of = [&](int col) {   // of the largest maximum
+		float b = sm_b[0][col];
 #pragma unroll
 		for (int w = 1; w < kAttnWarps; w++)
-			m = fmaxf(m, sm_m[w][col]);
-		return m;
+			b = fminf(b, sm_b[w][col]);
+		return b;
 	};
 	constexpr int OS = HL + 4;
 	float *ob = reinterpret_cast<float *>(smem);
 #pragma unroll
 	for (int nt = 0; nt < NT; nt++) {
 		const int col = nt * 8 + 2 * c;
-		const float f0 = ex2(m0[nt] - top_of(col)), f1 = ex2(m1[nt] - top_of(col + 1));
+		const float f0 = ex2(bias_of(col) - b0[nt]), f1 = ex2(bias_of(col + 1) - b1[nt]);
 		float *o0 = ob + (warp * COLS + col) * OS, *o1 = o0 + OS;
 #pragma unroll
 		for (int k = 0; k < 2 * NB; k++) {
-			const float iv = 1.0f / rv[k / 2];
+			const float iv = (k & 1 ? kCodeUnit / 16 : kCodeUnit) / half_of(v_fac[k / 4], k / 2 & 1);
 			const int e = 32 * (k / 2) + 16 * (k & 1) + 2 * g;
 			*reinterpret_cast<float2 *>(o0 + e) =
 				make_float2(o[k][nt][0] * f0 * iv, o[k][nt][2] * f0 * iv);
@@ -837,12 +936,12 @@ __global__ void __launch_bounds__(kAttnThreads) kv_attn_kernel(AttnArgs a)
 	for (int i = threadIdx.x; i < it.rows * (HL / 4); i += kAttnThreads) {
 		const int r = i / (HL / 4), e = i % (HL / 4) * 4;
 		const int col = SPLIT ? r / RPN * 8 + 2 * (r % RPN) : r;
-		const float m = top_of(col);
+		const float b = bias_of(col);
 		float l = 0.0f;
 		float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
 		for (int w = 0; w < kAttnWarps; w++) {
-			l += sm_l[w][col] * ex2(sm_m[w][col] - m);
+			l += sm_l[w][col] * ex2(b - sm_b[w][col]);
 #pragma unroll
 			for (int h = 0; h < (SPLIT ? 2 : 1); h++) {
 				const float4 x =
@@ -857,48 +956,100 @@ __global__ void __launch_bounds__(kAttnThreads) kv_attn_kernel(AttnArgs a)
 			float *pp = a.part + ((int64_t)blockIdx.x * RPT + r) * OS;
 			*reinterpret_cast<float4 *>(pp + e) = v;
 			if (e == 0)
-				*reinterpret_cast<float2 *>(pp + HL) = make_float2(m, l);
+				*reinterpret_cast<float2 *>(pp + HL) = make_float2(b, l);
 		} else {
-			write_row<T>(a, it, r, e, v, m, l, e == 0);
+			write_row<T>(a, it, r, e, v, b, l, e == 0);
 		}
 	}
 }
 
-// one tile of query rows with several runs: their sums joined, a warp a row
+// The runs of a query row joined: grid (query tile, row of it), the warps
+// taking the runs in turn.  A few dependent loads long, so the sums of a warp's
+// first runs leave before the factors are known.
 template <typename T, int HL, int RPT>
 __global__ void __launch_bounds__(kAttnThreads) kv_merge_kernel(AttnArgs a)
 {
-	constexpr int OS = HL + 4, E4 = HL / 4;   // float4s of a row
+	constexpr int OS = HL + 4, E4 = HL / 4;                  // float4s of a row
+	constexpr int W = E4 < 32 ? E4 : 32, SIDE = 32 / W, NV = E4 / W;
+	constexpr int BATCH = 4;
+	__shared__ float4 red[kAttnWarps][E4];
 	Item it;
 	const bool mine = find_item<RPT, false>(a, blockIdx.x, it) && it.runs > 1;
 	griddep_wait();   // the runs are written
-	if (!mine)
+	const int r = blockIdx.y;
+	if (!mine || r >= it.rows)
 		return;
 	const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 	const int64_t step = (int64_t)a.KVH * RPT * OS;   // between the runs of a tile
-	for (int r = warp; r < it.rows; r += kAttnWarps) {
-		const float *pp = a.part + ((int64_t)it.first * RPT + r) * OS;
-		float m = -3.0e38f;
-		for (int s = lane; s < it.runs; s += 32)
-			m = fmaxf(m, pp[s * step + HL]);
-		m = warp_max(m);
-		float l = 0.0f;
-		for (int s = lane; s < it.runs; s += 32)
-			l += pp[s * step + HL + 1] * ex2(pp[s * step + HL] - m);
-		l = warp_sum(l);
-		for (int e = lane; e < E4; e += 32) {
-			float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-			for (int s = 0; s < it.runs; s++) {
-				const float f = ex2(pp[s * step + HL] - m);
-				const float4 x = *reinterpret_cast<const float4 *>(pp + s * step + 4 * e);
-				v.x = fmaf(x.x, f, v.x);
-				v.y = fmaf(x.y, f, v.y);
-				v.z = fmaf(x.z, f, v.z);
-				v.w = fmaf(x.w, f, v.w);
-			}
-			write_row<T>(a, it, r, 4 * e, v, m, l, e == 0);
+	const float *pp = a.part + ((int64_t)it.first * RPT + r) * OS;
+	const int s0 = warp * SIDE + lane / W, e = lane % W * 4;
+	constexpr int ds = kAttnWarps * SIDE;
+	float4 x[BATCH][NV];
+	float xb[BATCH];
+	auto load = [&](int s) {
+#pragma unroll
+		for (int k = 0; k < BATCH; k++) {
+			const float *p = pp + (s + k * ds) * step;
+			const bool in = s + k * ds < it.runs;
+			xb[k] = in ? p[HL] : kNoMax;
+#pragma unroll
+			for (int v = 0; v < NV; v++)
+				x[k][v] = in ? *reinterpret_cast<const float4 *>(p + e + 4 * W * v)
+					     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 		}
+	};
+	load(s0);
+	float b = kNoMax;
+	for (int s = lane; s < it.runs; s += 32)
+		b = fminf(b, pp[s * step + HL]);
+	b = -warp_max(-b);
+	float l = 0.0f;
+	for (int s = lane; s < it.runs; s += 32)
+		l += pp[s * step + HL + 1] * ex2(b - pp[s * step + HL]);
+	l = warp_sum(l);
+	float4 o[NV];
+#pragma unroll
+	for (int v = 0; v < NV; v++)
+		o[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+	for (int s = s0;; load(s)) {
+#pragma unroll
+		for (int k = 0; k < BATCH; k++) {
+			const float f = ex2(b - xb[k]);
+#pragma unroll
+			for (int v = 0; v < NV; v++) {
+				o[v].x = fmaf(x[k][v].x, f, o[v].x);
+				o[v].y = fmaf(x[k][v].y, f, o[v].y);
+				o[v].z = fmaf(x[k][v].z, f, o[v].z);
+				o[v].w = fmaf(x[k][v].w, f, o[v].w);
+			}
+		}
+		s += BATCH * ds;
+		if (s - lane / W >= it.runs)
+			break;
+	}
+#pragma unroll
+	for (int v = 0; v < NV; v++) {
+		if (SIDE == 2) {
+			o[v].x += __shfl_xor_sync(0xffffffffu, o[v].x, 16);
+			o[v].y += __shfl_xor_sync(0xffffffffu, o[v].y, 16);
+			o[v].z += __shfl_xor_sync(0xffffffffu, o[v].z, 16);
+			o[v].w += __shfl_xor_sync(0xffffffffu, o[v].w, 16);
+		}
+		if (lane < W)
+			red[warp][lane + W * v] = o[v];
+	}
+	__syncthreads();
+	if (threadIdx.x < E4) {
+		float4 v = red[0][threadIdx.x];
+#pragma unroll
+		for (int w = 1; w < kAttnWarps; w++) {
+			const float4 y = red[w][threadIdx.x];
+			v.x += y.x;
+			v.y += y.y;
+			v.z += y.z;
+			v.w += y.w;
+		}
+		write_row<T>(a, it, r, 4 * threadIdx.x, v, b, l, threadIdx.x == 0);
 	}
 }
 
@@ -906,6 +1057,7 @@ __global__ void __launch_bounds__(kAttnThreads) kv_merge_kernel(AttnArgs a)
 // the sizes that a launch is planned with, from the call's bounds alone
 struct Plan {
 	int nt = 1, rpt = 8;     // column tiles, query rows of an item
+	int rows = 8;            // rows of them that can be in use
 	int64_t tiles = 0;       // at most so many query tiles x KV heads
 	int64_t items = 0;       // and items
 	int target = 0;
@@ -925,13 +1077,20 @@ Plan plan_of(const moe_kv_cache *c, const moe_kv_batch *b, int64_t H, bool fp32)
 	const int64_t by_seq = b->n_seqs * ((rows + p.rpt - 1) / p.rpt);
 	const int64_t by_token = b->n_tokens * G / p.rpt + b->n_seqs;
 	p.tiles = KVH * (by_seq < by_token ? by_seq : by_token);
-	p.target = 6 * sm_count();
-	p.split = p.tiles < 4 * (int64_t)p.target;
+	p.rows = (int)(rows < p.rpt ? rows : p.rpt);
+	// items for whole waves of resident CTAs (4 an SM, fewer for wide tiles), the
+	// runs' remainders among them (a remainder a query tile at most)
+	const int64_t wave = (int64_t)sm_count() * (HL * p.nt <= 128 ? 4 : 2);
+	int64_t want = wave - p.tiles;
+	while (want < wave / 2)
+		want += wave;
+	p.target = (int)want;
+	p.split = p.tiles < 4 * wave;
 	p.items = p.tiles;
 	if (p.split) {
 		const int64_t longest = (b->max_kv + kAttnTile - 1) / kAttnTile;
 		const int64_t capped = p.tiles * longest / kRunMax + 1;
-		p.items += capped > p.target ? capped : p.target;
+		p.items += 1 + (capped > p.target ? capped : p.target);
 		p.part_bytes = (size_t)(p.items * p.rpt * (HL + 4) * 4);
 	}
 	return p;
@@ -950,7 +1109,7 @@ cudaError_t launch_attn_as(const AttnArgs &a, const Plan &p, cudaStream_t st)
 	if (!p.split)
 		return cudaSuccess;
 	cudaLaunchConfig_t cfg{};
-	cfg.gridDim = dim3((unsigned)p.tiles);
+	cfg.gridDim = dim3((unsigned)p.tiles, p.rows < RPT ? p.rows : RPT);
 	cfg.blockDim = dim3(kAttnThreads);
 	cfg.stream = st;
 	cudaLaunchAttribute at[1];

@@ -167,12 +167,13 @@ def attention_bounds(dtype, size, vmax, n_rows, out, lse):
     A weight: exp of that, of an argument rounded to 2^-23 of its size, and of the
     2-ulp exponential: 2^-20 size + 2^-20; it moves numerator and denominator.
     Weighted sums: a chain of products 16 rows long each (n / 64 of them or fewer a
-    warp, 2^-23), joined over 4 warps and the runs.  16-bit rows: weights
-    rounded to fp16 (2^-11), the result to its type (half of eps)."""
+    warp, 2^-23), joined over 4 warps and the runs.  16-bit rows: a weight is
+    rounded to fp16 before and after its row's scale multiplies it (2^-11 each), the
+    result to its type (half of eps)."""
     e = 2.0 ** -20 * size[..., None] + 2.0 ** -20
     tol = vmax * (2 * e + (n_rows / 64 + 16) * 2.0 ** -23)
     if dtype != torch.float32:
-        tol = tol + vmax * 2.0 ** -11
+        tol = tol + vmax * 2 * 2.0 ** -11
     tol = tol + np.abs(out) * torch.finfo(dtype).eps / 2 + float(torch.finfo(dtype).tiny)
     tol_lse = 2.0 ** -20 * size + 2.0 ** -20 * (1 + np.abs(np.where(np.isfinite(lse), lse, 0)))
     return tol, tol_lse
