@@ -107,7 +107,8 @@ inline int check_rows(const char *what, const char *name, const moe_rows *r, int
 	if (r->type != type)
 		return kv_fail(MOE_ERR_UNSUPPORTED, "%s: %s has type %d beside %d", what, name, r->type,
 			       type);
-	if (r->n_heads <= 0 || r->n_heads > 65535 || (n_heads > 0 && r->n_heads != n_heads))
+	if (r->n_heads <= 0 || r->n_heads > (1 << 19) / head_len ||
+	    (n_heads > 0 && r->n_heads != n_heads))
 		return kv_fail(MOE_ERR_INVALID, "%s: %s has %lld heads", what, name,
 			       (long long)r->n_heads);
 	if ((uintptr_t)r->data % row_type_bytes(r->type))
@@ -221,37 +222,52 @@ __device__ __forceinline__ int find_seq(const int32_t *q_start, int B, int t)
 	return lo;
 }
 
-// where token t's row lies: its sequence's cache row, page and row of the
-// page; false (and the error word) if the arrays are out of range, silently
-// for padding
+// where a token's row lies: its sequence's cache row, page and row of the page;
+// not ok (and the error word) if the arrays are out of range, silently for padding
 struct TokenRow {
-	int row, page, at;
+	int ok, row, page, at;
 };
-__device__ __forceinline__ bool find_row(const BatchArgs &a, int t, TokenRow &r)
+// by a warp: lane l's is token t0 + l (l < n).  One search finds the first token's
+// sequence; the others lie in it or in the next ones.
+__device__ __forceinline__ TokenRow find_rows(const BatchArgs &a, int t0, int n)
 {
-	const int b = find_seq(a.q_start, a.B, t);
+	const int lane = threadIdx.x % 32, t = t0 + lane;
+	TokenRow r{0, 0, 0, 0};
+	int b = find_seq(a.q_start, a.B, t0);
+	if (lane >= n)
+		return r;
+	int s1 = b < a.B ? a.q_start[b + 1] : 0;
+	for (; b < a.B && s1 <= t; s1 = b < a.B ? a.q_start[b + 1] : 0)
+		b++;
 	if (b >= a.B)
-		return false;
-	const int s0 = a.q_start[b], s1 = a.q_start[b + 1], kv = a.kv_len[b];
+		return r;
+	const int s0 = a.q_start[b], kv = a.kv_len[b];
 	r.row = kv - (s1 - t);
 	if (s0 < 0 || s0 > t || s1 <= t || s1 > a.T || s1 - s0 > a.max_q || kv < s1 - s0 ||
 	    kv > a.max_kv) {
-		if (threadIdx.x == 0)
-			atomicOr(a.err, kKvErrBatch);
-		return false;
+		atomicOr(a.err, kKvErrBatch);
+		return r;
 	}
 	r.page = a.table[b * a.table_stride + (r.row >> a.page_log2)];
 	r.at = r.row & ((1 << a.page_log2) - 1);
 	if (r.page < 0 || r.page >= a.n_pages) {
-		if (threadIdx.x == 0)
-			atomicOr(a.err, kKvErrPage);
-		return false;
+		atomicOr(a.err, kKvErrPage);
+		return r;
 	}
-	return true;
+	r.ok = 1;
+	return r;
 }
 
-template <typename T>
-constexpr int kVec = 16 / (int)sizeof(T);   // values of a 16-byte vector
+// by a warp of the first CTA: sequences that no token leads to (a q_start that
+// falls names none) are reported too
+__device__ __forceinline__ void check_sequences(const BatchArgs &a)
+{
+	bool bad = threadIdx.x % 32 == 0 && a.q_start[0] != 0;
+	for (int b = threadIdx.x % 32; b < a.B; b += 32)
+		bad |= a.q_start[b + 1] < a.q_start[b] || a.q_start[b + 1] > a.T;
+	if (bad)
+		atomicOr(a.err, kKvErrBatch);
+}
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
@@ -264,47 +280,63 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
 	return __float2bfloat16_rn(v);
 }
 
-template <typename T>
-union Vec16 {
-	uint4 u;
-	T v[kVec<T>];
-	__device__ Vec16() {}
+// N values side by side as they lie in memory: 16-byte accesses (VEC) or single
+// ones.  Loads in flight hold no more registers than they bring bytes.
+template <typename T, int N, bool VEC>
+struct Raw {
+	static_assert(!VEC || N * sizeof(T) % 16 == 0, "whole vectors");
+	union {
+		T v[N];
+		uint32_t w[(N * sizeof(T) + 3) / 4];
+		uint4 u[(N * sizeof(T) + 15) / 16];
+	};
+	__device__ Raw() {}
+	__device__ void load(const T *p)
+	{
+		if constexpr (VEC) {
+#pragma unroll
+			for (int i = 0; i < (int)(N * sizeof(T) / 16); i++)
+				u[i] = reinterpret_cast<const uint4 *>(p)[i];
+		} else {
+#pragma unroll
+			for (int i = 0; i < N; i++)
+				v[i] = p[i];
+		}
+	}
+	__device__ void store(T *p) const
+	{
+		if constexpr (VEC) {
+#pragma unroll
+			for (int i = 0; i < (int)(N * sizeof(T) / 16); i++)
+				reinterpret_cast<uint4 *>(p)[i] = u[i];
+		} else {
+#pragma unroll
+			for (int i = 0; i < N; i++)
+				p[i] = v[i];
+		}
+	}
+	__device__ void get(float (&f)[N]) const
+	{
+#pragma unroll
+		for (int i = 0; i < N; i++)
+			f[i] = to_f32(v[i]);
+	}
+	__device__ void set(const float (&f)[N])
+	{
+#pragma unroll
+		for (int i = 0; i < N; i++)
+			v[i] = from_f32<T>(f[i]);
+	}
+	// another lane's
+	__device__ Raw from_lane(int lane) const
+	{
+		Raw r;
+#pragma unroll
+		for (int i = 0; i < (int)(N * sizeof(T) / 4); i++)
+			r.w[i] = __shfl_sync(0xffffffffu, w[i], lane);
+		return r;
+	}
 };
-
-// N consecutive values: one 16-byte access (VEC, N = kVec<T>) or N single ones
-template <typename T, int N, bool VEC>
-__device__ __forceinline__ void load_n(const T *p, float (&f)[N])
-{
-	if constexpr (VEC) {
-		static_assert(N == kVec<T>, "one vector");
-		Vec16<T> x;
-		x.u = *reinterpret_cast<const uint4 *>(p);
-#pragma unroll
-		for (int i = 0; i < N; i++)
-			f[i] = to_f32(x.v[i]);
-	} else {
-#pragma unroll
-		for (int i = 0; i < N; i++)
-			f[i] = to_f32(p[i]);
-	}
-}
-
-template <typename T, int N, bool VEC>
-__device__ __forceinline__ void store_n(T *p, const float (&f)[N])
-{
-	if constexpr (VEC) {
-		static_assert(N == kVec<T>, "one vector");
-		Vec16<T> x;
-#pragma unroll
-		for (int i = 0; i < N; i++)
-			x.v[i] = from_f32<T>(f[i]);
-		*reinterpret_cast<uint4 *>(p) = x.u;
-	} else {
-#pragma unroll
-		for (int i = 0; i < N; i++)
-			p[i] = from_f32<T>(f[i]);
-	}
-}
 
 // ---------------------------------------------------------------- rotation
 struct RopeArgs {
@@ -325,16 +357,14 @@ inline RopeArgs rope_args(const moe_rope *r)
 	return a;
 }
 
-// cosine and sine of every pair at a position, by the CTA's threads: the
-// sum of the two tables' angles, (cos + i sin) multiplied in 64 bits, so
-// the fp32 result is the 64-bit one rounded
-__device__ __forceinline__ void rope_angles(const RopeArgs &r, int pos, float2 *cs)
+// cosine and sine of pair i at a position: the sum of the two tables' angles,
+// (cos + i sin) multiplied in 64 bits, so the fp32 result is the 64-bit one
+// rounded
+__device__ __forceinline__ float2 rope_angle(const RopeArgs &r, int pos, int i)
 {
-	for (int i = threadIdx.x; i < r.half; i += blockDim.x) {
-		const double2 a = r.lo[(int64_t)(pos % kRopeLow) * r.half + i];
-		const double2 b = r.hi[(int64_t)(pos / kRopeLow) * r.half + i];
-		cs[i] = make_float2((float)(a.x * b.x - a.y * b.y), (float)(a.x * b.y + a.y * b.x));
-	}
+	const double2 a = r.lo[(int64_t)(pos % kRopeLow) * r.half + i];
+	const double2 b = r.hi[(int64_t)(pos / kRopeLow) * r.half + i];
+	return make_float2((float)(a.x * b.x - a.y * b.y), (float)(a.x * b.y + a.y * b.x));
 }
 
 // each product and the sum rounded once (rope_apply's operations, nn.c:192-219)
@@ -373,45 +403,322 @@ inline Heads<T> heads_of(const moe_rows *in, const moe_rows *out)
 	return h;
 }
 
-// A head's values in items that one thread reads, turns and writes whole, so
-// that an output may be its input.  PAIRS: N values side by side.  HALVES: the
-// first items hold N values of each half (their partners), the rest N values
-// behind the turning ones.
-template <int N, int LAYOUT>
-struct RopeItem {
-	int e0, e1;   // first value, and the partners' (HALVES: -1 behind rot)
-	__device__ RopeItem(int i, int half)
+// j / n for j * n < 2^32 by the high half of a product; or (zero) 0
+struct FastDiv {
+	unsigned n = 1, m = 0;
+	FastDiv() {}
+	explicit FastDiv(unsigned n_, bool zero = false)
+		: n(zero ? 2 : n_), m(n_ > 1 && !zero ? (unsigned)(0x100000000ull / n_) + 1 : 0)
 	{
-		const int pairs = LAYOUT == MOE_ROPE_HALVES ? half / N : 0;
-		if (LAYOUT == MOE_ROPE_PAIRS) {
-			e0 = i * N;
-			e1 = -1;
-		} else if (i < pairs) {
-			e0 = i * N;
-			e1 = half + i * N;
+	}
+	__device__ unsigned div(unsigned j) const { return n > 1 ? __umulhi(j, m) : j; }
+};
+
+// How a kernel takes the turning pairs: beside each other; in two halves whose
+// 8-value vectors are partners (half % 8 == 0; a head's vectors in lanes of one
+// warp); or in halves of any size, value by value
+enum { kTurnPairs = 0, kTurnHalves = 1, kTurnAny = 2 };
+inline int turn_of(int layout, int half)
+{
+	return layout == MOE_ROPE_PAIRS ? kTurnPairs : half % 8 == 0 ? kTurnHalves : kTurnAny;
+}
+
+// A lane's 8 values e0 .. of any head of a token, with the token's angles for them in
+// registers (a row's vectors stand in consecutive lanes, so every row that a lane
+// takes part in has the same place for it).
+template <int TURN>
+struct Turn8 {
+	static_assert(TURN != kTurnAny, "by value");
+	static constexpr int kAngles = TURN == kTurnPairs ? 4 : 8;
+	float2 c[kAngles];
+	int turning;   // PAIRS: of the 4 pairs; HALVES: all or none
+	int from;      // HALVES: the partners' lane
+	bool low;      // HALVES: in the first half
+	__device__ Turn8(int e0, int half)
+	{
+		if (TURN == kTurnPairs) {
+			turning = min(max(half - e0 / 2, 0), 4);
+			low = true;
+			from = 0;
 		} else {
-			e0 = 2 * half + (i - pairs) * N;
-			e1 = -1;
+			const int lane = threadIdx.x % 32;
+			low = e0 < half;
+			turning = e0 < 2 * half ? 8 : 0;
+			from = !turning ? lane : low ? lane + half / 8 : lane - half / 8;
 		}
 	}
-	__host__ __device__ static int per_head(int head_len, int half)
+	__device__ void angles(const float2 *cs, int e0, int half)
 	{
-		return LAYOUT == MOE_ROPE_PAIRS ? head_len / N : head_len / N - half / N;
-	}
-	__device__ void apply(float (&x)[N], float (&y)[N], const float2 *cs, int half) const
-	{
-		if (LAYOUT == MOE_ROPE_PAIRS) {
-			if constexpr (N >= 2) {
+		const float2 *p = cs + (TURN == kTurnPairs ? e0 / 2 : low ? e0 : e0 - half);
 #pragma unroll
-				for (int k = 0; k < N; k += 2)
-					if ((e0 + k) / 2 < half)
-						turn(x[k], x[k + 1], cs[(e0 + k) / 2]);
+		for (int k = 0; k < kAngles; k++)
+			if (k < turning)
+				c[k] = p[k];
+		if (TURN == kTurnHalves && low) {
+			// the low value's partner counts negatively: a + (-b) is a - b
+#pragma unroll
+			for (int k = 0; k < kAngles; k++)
+				c[k].y = -c[k].y;
+		}
+	}
+	// every lane of the warp calls it: partners come from their lanes, so an output
+	// may be its input
+	template <typename R>
+	__device__ void apply(const R &x, float (&f)[8]) const
+	{
+		x.get(f);
+		if constexpr (TURN == kTurnPairs) {
+#pragma unroll
+			for (int k = 0; k < 4; k++)
+				if (k < turning)
+					turn(f[2 * k], f[2 * k + 1], c[k]);
+		} else {
+			float g[8];
+			x.from_lane(from).get(g);
+			if (turning) {
+#pragma unroll
+				for (int k = 0; k < 8; k++)
+					f[k] = __fadd_rn(__fmul_rn(f[k], c[k].x), __fmul_rn(g[k], c[k].y));
 			}
-		} else if (e1 >= 0) {
-#pragma unroll
-			for (int k = 0; k < N; k++)
-				turn(x[k], y[k], cs[e0 + k]);
 		}
+	}
+};
+
+// The rounds of a token, a round being 32 lanes of whole rows: a group's tokens go to
+// the CTA's warps in turn; with fewer tokens than warps (1, 2, 4) a token's rounds
+// are dealt to several warps, and over the grid's slices.
+struct Rounds {
+	int token, token_step;   // first and next of the warp's tokens
+	int first, step_log2;    // of a token's rounds
+	__device__ __forceinline__ Rounds(const struct TokenSplit &s, int slice);
+	__device__ __forceinline__ int step() const { return 1 << step_log2; }
+	// the first of the warp's rounds of a sort of rows that `before` rounds precede
+	__device__ __forceinline__ int start(int before) const
+	{
+		const int d = before - first;
+		return d <= 0 ? -d : -d & (step() - 1);
+	}
+};
+
+// value i of a head's first half and its partner, or a value behind the turning
+// ones: an item of kTurnAny
+template <typename T>
+struct PairItem {
+	T a, b;
+	__device__ static int first(int i, int half) { return i < half ? i : i + half; }
+	__device__ void load(const T *head, int i, int half)
+	{
+		a = head[first(i, half)];
+		if (i < half)
+			b = head[i + half];
+	}
+	__device__ void turn_store(T *head, int i, const float2 *cs, int half) const
+	{
+		if (i < half) {
+			float x = to_f32(a), y = to_f32(b);
+			turn(x, y, cs[i]);
+			head[i] = from_f32<T>(x);
+			head[i + half] = from_f32<T>(y);
+		} else {
+			head[i + half] = a;
+		}
+	}
+};
+
+// How a packed batch is cut into CTAs of 8 warps (a token's items are `rounds` warps
+// of them): as many tokens to a CTA (up to kGroupTokens, and 2048 angles) as leave one
+// wave of resident CTAs, so that the look-ups and angles that a CTA waits for are
+// paid once for much work; few tokens: several warps and CTAs a token.  Powers of
+// two, for the divisions that a decode step would wait for.
+constexpr int kGroupTokens = 32;
+struct TokenSplit {
+	int tokens;       // of a CTA: 1, 2, 4 or a multiple of 8
+	int share_log2;   // warps of a token: 8, 4, 2 or 1
+	int slices_log2;  // CTAs of a token
+};
+inline TokenSplit split_tokens(int64_t n_tokens, int64_t rounds, int half)
+{
+	const int64_t wave = 4 * (int64_t)sm_count();
+	int64_t tokens = (n_tokens + wave - 1) / wave;
+	tokens = tokens < kGroupTokens ? tokens : kGroupTokens;
+	while (tokens > 1 && tokens * half > 2048)
+		tokens--;
+	if (tokens > 1) {
+		tokens = tokens < 3 ? 2 : tokens < 7 ? 4 : (tokens + 4) / 8 * 8;
+		return {(int)tokens, tokens == 2 ? 2 : tokens == 4 ? 1 : 0, 0};
+	}
+	int y = 0;
+	while (y < 15 && (int64_t)8 << y < rounds && n_tokens << (y + 1) <= 2 * wave)
+		y++;
+	return {1, 3, y};
+}
+
+__device__ __forceinline__ Rounds::Rounds(const TokenSplit &s, int slice)
+{
+	const int warp = threadIdx.x / 32;
+	token = warp >> s.share_log2;
+	token_step = 8 >> s.share_log2;
+	first = (slice << s.share_log2) + (warp & ((1 << s.share_log2) - 1));
+	step_log2 = s.share_log2 + s.slices_log2;
+}
+
+// A warp's rows in flight to slots of its own in shared memory, kDepth rounds of them:
+// loads that hold no registers, so that a warp keeps 3 KB on the way whatever its
+// work needs (96 KB an SM).  Rounds come out in the order in which they went in.  A
+// lane gets 8 values side by side; those of fp32 rows are 32 bytes, which reach
+// memory as two times 16 that neighbouring lanes hold together (each 32-byte sector
+// once).  Rows that are not 16-byte aligned are read where they come out.
+template <typename T, bool VEC>
+struct RowStream {
+	static constexpr int kParts = 8 * sizeof(T) / 16, kDepth = 12 / (int)sizeof(T);
+	static constexpr int kWarpBytes = VEC ? kDepth * kParts * 512 : 0;
+	uint32_t mine, part;   // the lane's 8 values of a slot, its 16 bytes of a row's first part
+	int across, jump;      // bytes from part to part, and from the values to part 0 in memory
+	int in = 0, out = 0;
+	const T *next[VEC ? 1 : kDepth];
+	__device__ RowStream(uint8_t *slots, int row_lanes)
+	{
+		const uint32_t base = (uint32_t)__cvta_generic_to_shared(slots) + threadIdx.x / 32 * kWarpBytes;
+		const int lane = threadIdx.x % 32, j = lane & (row_lanes - 1);
+		mine = base + lane * 16 * kParts;
+		across = kParts == 1 ? 0 : 16 * row_lanes;
+		jump = kParts == 1 ? 0 : -16 * j;
+		part = mine + jump;
+	}
+	__device__ __forceinline__ void push(const T *p)   // NULL: no row
+	{
+		if constexpr (VEC) {
+			if (p) {
+				const uint8_t *q = reinterpret_cast<const uint8_t *>(p) + jump;
+#pragma unroll
+				for (int i = 0; i < kParts; i++)
+					asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+							     part + in * (512 * kParts) + i * across),
+						     "l"(q + i * across)
+						     : "memory");
+			}
+			asm volatile("cp.async.commit_group;" ::: "memory");
+			in = in + 1 == kDepth ? 0 : in + 1;
+		} else {
+#pragma unroll
+			for (int i = 0; i + 1 < kDepth; i++)
+				next[i] = next[i + 1];
+			next[kDepth - 1] = p;
+		}
+	}
+	__device__ __forceinline__ void idle()   // keeps the count of groups in step
+	{
+		if constexpr (VEC)
+			asm volatile("cp.async.commit_group;" ::: "memory");
+		else
+			push(nullptr);
+	}
+	__device__ __forceinline__ void pop(Raw<T, 8, VEC> &x)
+	{
+		if constexpr (VEC) {
+			asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+			if (kParts > 1)
+				__syncwarp();   // the other lanes' parts
+#pragma unroll
+			for (int i = 0; i < kParts; i++)
+				asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+					     : "=r"(x.u[i].x), "=r"(x.u[i].y), "=r"(x.u[i].z), "=r"(x.u[i].w)
+					     : "r"(mine + out * (512 * kParts) + 16 * i)
+					     : "memory");
+			out = out + 1 == kDepth ? 0 : out + 1;
+			if (kParts > 1)
+				__syncwarp();   // read by all before a next row overwrites it
+		} else if (next[0]) {
+			x.load(next[0]);
+		}
+	}
+	// the round popped last, written to p (NULL: nothing) before the next push
+	__device__ __forceinline__ void store(const Raw<T, 8, VEC> &x, T *p)
+	{
+		if constexpr (VEC && kParts > 1) {
+			const uint32_t slot = (out == 0 ? kDepth - 1 : out - 1) * (512 * kParts);
+#pragma unroll
+			for (int i = 0; i < kParts; i++)
+				asm volatile("st.shared.v4.u32 [%4], {%0, %1, %2, %3};" ::"r"(x.u[i].x),
+					     "r"(x.u[i].y), "r"(x.u[i].z), "r"(x.u[i].w),
+					     "r"(mine + slot + 16 * i)
+					     : "memory");
+			__syncwarp();
+#pragma unroll
+			for (int i = 0; i < kParts; i++) {
+				uint4 v;
+				asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+					     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+					     : "r"(part + slot + i * across)
+					     : "memory");
+				if (p)
+					*reinterpret_cast<uint4 *>(reinterpret_cast<uint8_t *>(p) + jump +
+								   i * across) = v;
+			}
+			__syncwarp();
+		} else if (p) {
+			x.store(p);
+		}
+	}
+	__device__ __forceinline__ void finish()
+	{
+		if constexpr (VEC)
+			asm volatile("cp.async.wait_group 0;" ::: "memory");
+	}
+};
+
+// A warp's rounds of one sort of rows of a token, in turn: round r's row of a lane is
+// row r * m + sub of heads.n
+template <typename T>
+struct RowWalk {
+	int row, rows, left, step_rows;   // the lane's next row, of how many; rounds left
+	__device__ __forceinline__ RowWalk(int n, int m_log2, int sub, int start, int step_log2)
+		: row((start << m_log2) + sub), rows(n)
+	{
+		const int rounds = (n + (1 << m_log2) - 1) >> m_log2;
+		left = rounds > start ? (rounds - start + (1 << step_log2) - 1) >> step_log2 : 0;
+		step_rows = 1 << (m_log2 + step_log2);
+	}
+	__device__ __forceinline__ bool has() const { return row < rows; }
+};
+
+// the same rows on their way, kDepth rounds ahead of the work
+template <typename T, bool VEC>
+struct RowReader {
+	RowStream<T, VEC> &stream;
+	RowWalk<T> w;
+	const T *p;
+	int64_t d;
+	__device__ __forceinline__ RowReader(RowStream<T, VEC> &s, const Heads<T> &h, int64_t token, int n,
+					     int m_log2, int sub, int e0, int start, int step_log2)
+		: stream(s), w(n, m_log2, sub, start, step_log2),
+		  p(h.in + token * h.in_ts + (int64_t)w.row * h.in_hs + e0), d((int64_t)w.step_rows * h.in_hs)
+	{
+	}
+	__device__ __forceinline__ void next()
+	{
+		if (w.left > 0) {
+			stream.push(w.has() ? p : nullptr);
+			w.left--;
+			w.row += w.step_rows;
+			p += d;
+		} else {
+			stream.idle();
+		}
+	}
+	__device__ __forceinline__ void begin()
+	{
+#pragma unroll
+		for (int i = 0; i < RowStream<T, VEC>::kDepth; i++)
+			next();
+	}
+	// the same rows begun by another reader
+	__device__ __forceinline__ void skip_begun()
+	{
+		const int n = min(w.left, RowStream<T, VEC>::kDepth);
+		w.left -= n;
+		w.row += n * w.step_rows;
+		p += n * d;
 	}
 };
 

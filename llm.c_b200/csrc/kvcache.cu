@@ -7,8 +7,8 @@
 namespace moe {
 namespace {
 
-constexpr int kAppendThreads = 256;
-constexpr int kAppendBatch = 2;   // items of a thread whose loads are in flight together
+constexpr int kAppendThreads = 256, kAppendCtas = 4;
+constexpr int kGatherBatch = 4;
 
 // address of a KV head's record of a page: K codes, K scales, V codes, V scales
 struct PageArgs {
@@ -28,10 +28,13 @@ PageArgs page_args(const moe_kv_cache *c)
 	return a;
 }
 
-__device__ __forceinline__ uint8_t *record(const PageArgs &a, int page, int head, int which)
+__device__ __forceinline__ int64_t record_bytes(const PageArgs &a)   // of a head's K, or V
 {
-	const int64_t half = ((int64_t)a.head_len / 2 + a.head_len / 16) << a.page_log2;
-	return a.pages + page * a.page_bytes + (2 * head + which) * half;
+	return (a.head_len / 2 + a.head_len / 16) << a.page_log2;
+}
+__device__ __forceinline__ uint8_t *record(const PageArgs &a, uint8_t *page, int head, int which)
+{
+	return page + (2 * head + which) * record_bytes(a);
 }
 
 template <typename T>
@@ -41,32 +44,35 @@ struct AppendArgs {
 	RopeArgs r;
 	const int32_t *pos;   // or NULL: the cache rows
 	Heads<T> q, k, v;     // k, v: inputs only; q.n 0: none
+	TokenSplit cut;
+	FastDiv half;         // pairs, to divide by
+	int per_log2;         // a row's lanes
+	FastDiv per_q;        // kTurnAny: a query head's items
 };
 
-// A lane's N values of a 32-value block, N / 32 of it in consecutive lanes:
-// the block's scale and codes (moe_kv_desc), two 4-bit codes to a byte with
-// the lane that holds the values 16 further on.  Lanes of the lower half
-// return the block's bytes sub * N .. sub * N + N - 1.
-template <int N>
-__device__ __forceinline__ void quantize_block(const float (&x)[N], __half &scale,
-					       uint32_t (&by)[N / 4])
+constexpr int kLanes = 4;   // of a 32-value block: 8 values each
+
+// A lane's 8 values of a block whose 4 lanes stand side by side: the block's scale
+// and codes (moe_kv_desc), two 4-bit codes to a byte with the lane that holds the
+// values 16 further on.  The two lower lanes return the block's bytes 0 .. 7 and
+// 8 .. 15.
+__device__ __forceinline__ void quantize_block(const float (&x)[8], __half &scale, uint32_t (&by)[2])
 {
-	constexpr int L = 32 / N;
 	float hi = x[0], lo = x[0];
 	bool bad = false;
 #pragma unroll
-	for (int k = 0; k < N; k++) {
+	for (int k = 0; k < 8; k++) {
 		hi = fmaxf(hi, x[k]);
 		lo = fminf(lo, x[k]);
 		bad |= !(fabsf(x[k]) <= 3.402823466e38f);
 	}
 #pragma unroll
-	for (int o = 1; o < L; o *= 2) {
+	for (int o = 1; o < kLanes; o *= 2) {
 		hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
 		lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
 	}
 	const unsigned any = __ballot_sync(0xffffffffu, bad);
-	bad = (any >> (threadIdx.x % 32 / L * L)) & ((1u << L) - 1);
+	bad = (any >> (threadIdx.x % 32 / kLanes * kLanes)) & ((1u << kLanes) - 1);
 	// the value of the largest magnitude takes code 0 (-8): a step of m / 8
 	// where a symmetric code would have m / 7
 	const float m = hi >= -lo ? hi : lo;
@@ -76,165 +82,215 @@ __device__ __forceinline__ void quantize_block(const float (&x)[N], __half &scal
 	if (d == 0.0f || bad)   // one zero: which zero m is depends on the order of its zeros
 		scale = __ushort_as_half(bad ? 0x7fff : 0);
 #pragma unroll
-	for (int w = 0; w < N / 4; w++) {
+	for (int w = 0; w < 2; w++) {
 		uint32_t c = 0;
 #pragma unroll
 		for (int k = 0; k < 4; k++) {
 			const int code = min(max(__float2int_rn(__fmul_rn(x[4 * w + k], inv)), -8), 7) + 8;
 			c |= (uint32_t)(bad ? 8 : code) << (8 * k);
 		}
-		by[w] = c | __shfl_xor_sync(0xffffffffu, c, L / 2) << 4;
+		by[w] = c | __shfl_xor_sync(0xffffffffu, c, kLanes / 2) << 4;
 	}
 }
 
-// grid (token, slice of its items): per token the query heads are turned
-// and written, then the key heads turned and quantized, the value heads
-// quantized; a warp has items of one sort.  Bound by bytes for prompts (q, k, v
-// in, q and 0.5625 bytes a value out) and by latency for decode batches:
-// the rows leave for the registers first, then come the sequence (a search
-// of two rounds), the angles and the page, each a dependent load.
-template <typename T, bool VEC, int LAYOUT>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendArgs<T> a)
+// The layout's 4-byte words of a pair of blocks (2 b, 2 b + 1), whose 8 lanes stand
+// side by side: a K word is 4 bytes of one block (word s of the lane's block, s the
+// lane's place in it), a V word 2 bytes of each block (word p, p the lane's place in
+// the pair).  So a row is written and read in whole words by neighbouring lanes.
+__device__ __forceinline__ int row_word_at(int b, int nb, bool isv)
 {
-	constexpr int N = kVec<T>, L = 32 / N;
-	constexpr int QN = VEC ? N : LAYOUT == MOE_ROPE_PAIRS ? 2 : 1;   // q's item
-	extern __shared__ float2 cs[];
-	const int t = blockIdx.x;
-	const int D = a.p.head_len, half = a.r.half, nb = D / 32;
-	const int per_q = RopeItem<QN, LAYOUT>::per_head(D, half);
-	const int nq = a.q.n * per_q, nq32 = (nq + 31) / 32 * 32;
-	const int per = D / N, nkv = a.p.KVH * per;   // items of the keys, and of the values
-	const int total = nq32 + 2 * nkv;
-	const int step = gridDim.y * kAppendThreads;
-	TokenRow row;
-	int pos = 0;
-	bool ready = false;
-	for (int i0 = blockIdx.y * kAppendThreads + threadIdx.x; __syncthreads_or(i0 < total);
-	     i0 += kAppendBatch * step) {
-		float x[kAppendBatch][N], y[kAppendBatch][N];
+	const int p = threadIdx.x % (2 * kLanes), s = threadIdx.x % kLanes;
+	return isv ? p * 2 * nb + 2 * (b & ~1) : s * 4 * nb + 4 * b;
+}
+
+// that word, out of the bytes that the blocks' lower lanes hold (8 each)
+__device__ __forceinline__ uint32_t row_word(const uint32_t (&by)[2], bool isv)
+{
+	const int lane = threadIdx.x % 32, p = lane % (2 * kLanes), s = lane % kLanes;
+	const int byte = isv ? 2 * p : 4 * s;
+	const int src = (isv ? lane - p : lane - s) + byte / 8;
+	const uint32_t x0 = __shfl_sync(0xffffffffu, by[0], src), x1 = __shfl_sync(0xffffffffu, by[1], src);
+	const int two = (src + kLanes) & 31;   // a V word's other block
+	const uint32_t y0 = __shfl_sync(0xffffffffu, by[0], two), y1 = __shfl_sync(0xffffffffu, by[1], two);
+	const uint32_t x = byte & 4 ? x1 : x0, y = byte & 4 ? y1 : y0;
+	return isv ? __byte_perm(x, y, byte & 2 ? 0x7632 : 0x5410) : x;
+}
+
+// the bytes that hold a lane's own 8 values out of the words
+__device__ __forceinline__ void row_bytes(uint32_t word, int b, bool isv, uint32_t (&by)[2])
+{
+	const int lane = threadIdx.x % 32, p = lane % (2 * kLanes), s = lane % kLanes;
 #pragma unroll
-		for (int u = 0; u < kAppendBatch; u++) {
-			const int i = i0 + u * step;
-			if (i < nq) {
-				const RopeItem<QN, LAYOUT> it(i % per_q, half);
-				const T *p = a.q.in + t * a.q.in_ts + (i / per_q) * a.q.in_hs;
-				float f[QN];
-				load_n<T, QN, VEC>(p + it.e0, f);
-#pragma unroll
-				for (int k = 0; k < QN; k++)
-					x[u][k] = f[k];
-				if (LAYOUT == MOE_ROPE_HALVES && it.e1 >= 0) {
-					load_n<T, QN, VEC>(p + it.e1, f);
-#pragma unroll
-					for (int k = 0; k < QN; k++)
-						y[u][k] = f[k];
-				}
-			} else if (i >= nq32 && i < total) {
-				const int j = i - nq32, isv = j >= nkv, jj = isv ? j - nkv : j;
-				const Heads<T> &h = isv ? a.v : a.k;
-				const int e0 = jj % per * N;
-				const T *p = h.in + t * h.in_ts + (jj / per) * h.in_hs;
-				load_n<T, N, VEC>(p + e0, x[u]);
-				if (LAYOUT == MOE_ROPE_HALVES && !isv && e0 < 2 * half) {
-					// the partners of a key's values: in the other half
-					if constexpr (VEC) {
-						load_n<T, N, VEC>(p + (e0 < half ? e0 + half : e0 - half), y[u]);
-					} else {
-#pragma unroll
-						for (int k = 0; k < N; k++) {
-							const int e = e0 + k;
-							y[u][k] = e < half ? to_f32(p[e + half])
-								  : e < 2 * half ? to_f32(p[e - half]) : 0.0f;
-						}
-					}
-				}
+	for (int i = 0; i < 2; i++) {
+		const int k4 = s % 2 * 2 + i;   // bytes 4 k4 .. of the block
+		const int src = isv ? lane - p + 2 * k4 : lane - s + k4;
+		const uint32_t x = __shfl_sync(0xffffffffu, word, src);
+		const uint32_t y = __shfl_sync(0xffffffffu, word, (src + 1) & 31);
+		by[i] = isv ? __byte_perm(x, y, b & 1 ? 0x7632 : 0x5410) : x;
+	}
+}
+
+// grid (token group, slice of a token's rounds): per token the query heads are turned
+// and written, then the key heads turned and quantized, the value heads quantized.
+// Bound by bytes for prompts (q, k, v in, q and 0.5625 bytes a value out) and by
+// latency for decode batches: the first rows leave for the registers, then come the
+// tokens' sequences (a search of two rounds), angles and pages, each a dependent
+// load.  A lane has 8 values of a row and the same place in every row it meets, so a
+// token's angles stay in its registers (kTurnAny: halves that are no multiple of 8,
+// value by value).
+template <typename T, bool VEC, int TURN>
+__global__ void __launch_bounds__(kAppendThreads, kAppendCtas) append_kernel(const __grid_constant__ AppendArgs<T> a)
+{
+	extern __shared__ uint4 smem[];
+	struct Token {
+		int ok, pos, at;
+		uint8_t *page;
+	};
+	__shared__ Token toks[kGroupTokens];
+	uint8_t *slots = reinterpret_cast<uint8_t *>(smem);
+	float2 *cs = reinterpret_cast<float2 *>(   // [token][pair]
+		slots + kAppendThreads / 32 * RowStream<T, VEC>::kWarpBytes);
+	const int half = a.r.half, D = a.p.head_len, nb = D / 32;
+	const int t0 = blockIdx.x * a.cut.tokens, nt = min(a.cut.tokens, a.b.T - t0);
+	const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+	const int ml = 5 - a.per_log2;   // rows of a round, log2
+	const int e0 = (lane & ((1 << a.per_log2) - 1)) * 8, sub = lane >> a.per_log2;
+	const Rounds rr(a.cut, blockIdx.y);
+	// (kTurnAny: the queries go by items of their own)
+	constexpr int Q = TURN == kTurnAny ? 0 : 1;
+	RowStream<T, VEC> stream(slots, 1 << a.per_log2);
+	const int q_rounds = Q ? (a.q.n + (1 << ml) - 1) >> ml : 0;
+	const int kv_rounds = (a.k.n + (1 << ml) - 1) >> ml;
+	const int starts[3] = {rr.first, rr.start(q_rounds), rr.start(q_rounds + kv_rounds)};
+	auto reader = [&](int s, int t) {
+		const Heads<T> &h = s == 0 ? a.q : s == 1 ? a.k : a.v;
+		const int n = t >= nt || (s == 0 && !Q) ? 0 : h.n;
+		return RowReader<T, VEC>(stream, h, t0 + t, n, ml, sub, e0, starts[s], rr.step_log2);
+	};
+	// the first rows leave before the tokens' places are known: of the first sort
+	// that the warp has rows of
+	const int early = reader(0, rr.token).w.left > 0 ? 0 : reader(1, rr.token).w.left > 0 ? 1 : 2;
+	{
+		RowReader<T, VEC> first = early == 0   ? reader(0, rr.token)
+					  : early == 1 ? reader(1, rr.token)
+						       : reader(2, rr.token);
+		first.begin();
+	}
+	if (warp == 0) {
+		TokenRow row = find_rows(a.b, t0, nt);
+		int pos = 0;
+		if (row.ok) {
+			pos = a.pos ? a.pos[t0 + lane] : row.row;
+			if (half && (pos < 0 || pos >= a.r.max_position)) {
+				row.ok = 0;
+				atomicOr(a.b.err, kKvErrPos);
 			}
 		}
-		if (!ready) {
-			if (!find_row(a.b, t, row))
-				return;   // the whole CTA: t is its own
-			pos = a.pos ? a.pos[t] : row.row;
-			if (half) {
-				if (pos < 0 || pos >= a.r.max_position) {
-					if (threadIdx.x == 0)
-						atomicOr(a.b.err, kKvErrPos);
-					return;
-				}
-				rope_angles(a.r, pos, cs);
-			}
-			__syncthreads();
-			ready = true;
+		if (lane < nt) {
+			toks[lane].ok = row.ok;
+			toks[lane].pos = pos;
+			toks[lane].at = row.at;
+			toks[lane].page = a.p.pages + (row.ok ? row.page * a.p.page_bytes : 0);
 		}
-#pragma unroll
-		for (int u = 0; u < kAppendBatch; u++) {
-			const int i = i0 + u * step;
-			if (i < nq32) {
-				if (i < nq) {
-					const RopeItem<QN, LAYOUT> it(i % per_q, half);
-					float f[QN], g[QN];
-#pragma unroll
-					for (int k = 0; k < QN; k++) {
-						f[k] = x[u][k];
-						g[k] = y[u][k];
-					}
-					it.apply(f, g, cs, half);
-					T *p = a.q.out + t * a.q.out_ts + (i / per_q) * a.q.out_hs;
-					store_n<T, QN, VEC>(p + it.e0, f);
-					if (LAYOUT == MOE_ROPE_HALVES && it.e1 >= 0)
-						store_n<T, QN, VEC>(p + it.e1, g);
-				}
-				continue;   // the whole warp: nq32 is a multiple of 32
+	} else if (warp == 1 && blockIdx.x == 0 && blockIdx.y == 0) {
+		check_sequences(a.b);
+	}
+	__syncthreads();
+	if (half) {
+		for (int p = threadIdx.x; p < nt * half; p += kAppendThreads) {
+			const int u = a.half.div(p);
+			if (toks[u].ok)
+				cs[p] = rope_angle(a.r, toks[u].pos, p - u * half);
+		}
+		__syncthreads();
+	}
+	const int b = e0 / 32;
+	const int64_t kv_bytes = record_bytes(a.p);
+	Turn8<Q ? TURN : kTurnPairs> tn(e0, half);
+	for (int t = rr.token; t < nt; t += rr.token_step) {
+		const bool good = toks[t].ok;
+		const int64_t tok = t0 + t;
+		const float2 *tcs = cs + t * half;
+		T *qo = a.q.out + tok * a.q.out_ts;
+		if constexpr (Q) {
+			if (good)
+				tn.angles(tcs, e0, half);
+			RowReader<T, VEC> q = reader(0, t);
+			RowWalk<T> w = q.w;
+			if (t == rr.token && early == 0)
+				q.skip_begun();
+			else
+				q.begin();
+			qo += e0 + (int64_t)w.row * a.q.out_hs;
+			const int64_t d = (int64_t)w.step_rows * a.q.out_hs;
+			for (; w.left > 0; w.left--, w.row += w.step_rows, qo += d) {
+				Raw<T, 8, VEC> x;
+				stream.pop(x);
+				float f[8];
+				tn.apply(x, f);
+				if (tn.turning)   // what does not turn keeps its bits
+					x.set(f);
+				stream.store(x, good && w.has() ? qo : nullptr);
+				q.next();
 			}
-			const bool in = i < total;   // a block's lanes are in together
-			const int j = in ? i - nq32 : 0, isv = j >= nkv, jj = isv ? j - nkv : j;
-			const int head = jj / per, e0 = jj % per * N;
-			if (!in) {
-#pragma unroll
-				for (int k = 0; k < N; k++)
-					x[u][k] = 0.0f;
+		} else if (good) {
+			const int items = a.q.n * a.per_q.n;
+			for (int j = rr.first * 32 + lane; j < items; j += rr.step() * 32) {
+				const int head = a.per_q.div(j), i = j - head * a.per_q.n;
+				PairItem<T> x;
+				x.load(a.q.in + tok * a.q.in_ts + head * a.q.in_hs, i, half);
+				x.turn_store(qo + head * a.q.out_hs, i, tcs, half);
 			}
-			if (!isv && in) {
-				if (LAYOUT == MOE_ROPE_PAIRS) {
+		}
+		const int at = toks[t].at;
+		const int codes_at = at * (D / 2), scale_at = ((D / 2) << a.p.page_log2) + (at * nb + b) * 2;
 #pragma unroll
-					for (int k = 0; k < N; k += 2)
-						if ((e0 + k) / 2 < half)
-							turn(x[u][k], x[u][k + 1], cs[(e0 + k) / 2]);
-				} else {
+		for (int isv = 0; isv < 2; isv++) {
+			RowReader<T, VEC> in = reader(1 + isv, t);
+			RowWalk<T> w = in.w;
+			if (t == rr.token && early == 1 + isv)
+				in.skip_begun();
+			else
+				in.begin();
+			uint8_t *rec = toks[t].page + (2 * w.row + isv) * kv_bytes;
+			const int64_t d = 2 * w.step_rows * kv_bytes;
+			const int word_at = codes_at + row_word_at(b, nb, isv);
+			for (; w.left > 0; w.left--, w.row += w.step_rows, rec += d) {
+				Raw<T, 8, VEC> x;
+				stream.pop(x);
+				float f[8];
+				if (Q && !isv)
+					tn.apply(x, f);
+				else
+					x.get(f);
+				in.next();
+				if (!Q && !isv && good && e0 < 2 * half && w.has()) {
+					const T *src = a.k.in + tok * a.k.in_ts + w.row * a.k.in_hs + e0;
 #pragma unroll
-					for (int k = 0; k < N; k++) {
-						const int e = e0 + k;
+					for (int i = 0; i < 8; i++) {
+						const int e = e0 + i;
+						if (e >= 2 * half)
+							break;
+						float g = to_f32(src[e < half ? i + half : i - half]);
 						if (e < half)
-							turn(x[u][k], y[u][k], cs[e]);
-						else if (e < 2 * half)
-							turn(y[u][k], x[u][k], cs[e - half]);
+							turn(f[i], g, tcs[e]);
+						else
+							turn(g, f[i], tcs[e - half]);
 					}
 				}
-			}
-			__half scale;
-			uint32_t by[N / 4];
-			quantize_block<N>(x[u], scale, by);
-			if (!in)
-				continue;
-			const int b = e0 / 32, sub = e0 % 32 / N;
-			uint8_t *rec = record(a.p, row.page, head, isv);
-			if (sub == 0)
-				reinterpret_cast<__half *>(rec + ((D / 2) << a.p.page_log2))[row.at * nb + b] = scale;
-			if (sub < L / 2) {
-				uint8_t *dst = rec + row.at * (D / 2);
-#pragma unroll
-				for (int w = 0; w < N / 4; w++) {
-					const int k4 = sub * (N / 4) + w;   // bytes 4 k4 .. of the block
-					if (!isv) {
-						*reinterpret_cast<uint32_t *>(dst + k4 * 4 * nb + 4 * b) = by[w];
-					} else {
-						uint16_t *d2 = reinterpret_cast<uint16_t *>(dst + 2 * k4 * 2 * nb + 2 * b);
-						d2[0] = (uint16_t)by[w];
-						d2[nb] = (uint16_t)(by[w] >> 16);
-					}
+				__half scale;
+				uint32_t by[2];
+				quantize_block(f, scale, by);
+				const uint32_t word = row_word(by, isv);
+				if (good && w.has()) {
+					if (lane % kLanes == 0)
+						*reinterpret_cast<__half *>(rec + scale_at) = scale;
+					*reinterpret_cast<uint32_t *>(rec + word_at) = word;
 				}
 			}
 		}
 	}
+	stream.finish();
 }
 
 template <typename T>
@@ -242,83 +298,137 @@ struct GatherArgs {
 	BatchArgs b;
 	PageArgs p;
 	Heads<T> k, v;   // outputs only; n 0: none
+	TokenSplit cut;
+	int per_log2, k_rounds, v_rounds;
 };
 
-// grid (token, slice): the values of the token's rows, code by code
+// grid (token group, slice of a token's rounds): the values of the tokens' rows, code
+// by code, kGatherBatch rounds in flight together
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kAppendThreads) gather_kernel(GatherArgs<T> a)
+__global__ void __launch_bounds__(kAppendThreads) gather_kernel(const __grid_constant__ GatherArgs<T> a)
 {
-	constexpr int N = kVec<T>;
-	const int t = blockIdx.x, D = a.p.head_len, nb = D / 32;
-	const int per = D / N, nk = a.k.n * per, total = nk + a.v.n * per;
-	TokenRow row;
-	if (!find_row(a.b, t, row))
-		return;
-	for (int i = blockIdx.y * kAppendThreads + threadIdx.x; i < total;
-	     i += gridDim.y * kAppendThreads) {
-		const int isv = i >= nk, j = isv ? i - nk : i;
-		const int head = j / per, e0 = j % per * N;
-		const int b = e0 / 32, k0 = e0 % 16, up = e0 % 32 >= 16;
-		const uint8_t *rec = record(a.p, row.page, head, isv);
-		const float d = __half2float(
-			reinterpret_cast<const __half *>(rec + ((D / 2) << a.p.page_log2))[row.at * nb + b]);
-		const uint8_t *src = rec + row.at * (D / 2);
-		float f[N];
-#pragma unroll
-		for (int w = 0; w < N / 4; w++) {
-			const int k4 = k0 / 4 + w;
-			uint32_t by;
-			if (!isv) {
-				by = *reinterpret_cast<const uint32_t *>(src + k4 * 4 * nb + 4 * b);
-			} else {
-				const uint16_t *s2 = reinterpret_cast<const uint16_t *>(src + 2 * k4 * 2 * nb + 2 * b);
-				by = s2[0] | (uint32_t)s2[nb] << 16;
-			}
-			by = up ? by >> 4 : by;
-#pragma unroll
-			for (int k = 0; k < 4; k++)
-				f[4 * w + k] = __fmul_rn((float)((int)(by >> (8 * k) & 15) - 8), d);
+	__shared__ uint8_t *page_of[kGroupTokens];
+	__shared__ int row_of[kGroupTokens];
+	const int D = a.p.head_len, nb = D / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+	const int t0 = blockIdx.x * a.cut.tokens, nt = min(a.cut.tokens, a.b.T - t0);
+	if (warp == 0) {
+		const TokenRow row = find_rows(a.b, t0, nt);
+		if (lane < nt) {
+			page_of[lane] = row.ok ? a.p.pages + row.page * a.p.page_bytes : nullptr;
+			row_of[lane] = row.at;
 		}
-		const Heads<T> &h = isv ? a.v : a.k;
-		store_n<T, N, VEC>(h.out + t * h.out_ts + head * h.out_hs + e0, f);
+	} else if (warp == 1 && blockIdx.x == 0 && blockIdx.y == 0) {
+		check_sequences(a.b);
+	}
+	__syncthreads();
+	const int rows = 32 >> a.per_log2;
+	const int e0 = (lane & ((1 << a.per_log2) - 1)) * 8, sub = lane >> a.per_log2, b = e0 / 32;
+	const Rounds rr(a.cut, blockIdx.y);
+	const int n = a.k_rounds + a.v_rounds;
+	for (int t = rr.token; t < nt; t += rr.token_step) {
+		uint8_t *page = page_of[t];
+		if (!page)
+			continue;
+		const int row = row_of[t];
+		T *ko = a.k.out + (int64_t)(t0 + t) * a.k.out_ts + e0;
+		T *vo = a.v.out + (int64_t)(t0 + t) * a.v.out_ts + e0;
+		for (int r0 = rr.first; r0 < n; r0 += kGatherBatch * rr.step()) {
+			uint32_t word[kGatherBatch];
+			__half scale[kGatherBatch];
+#pragma unroll
+			for (int u = 0; u < kGatherBatch; u++) {
+				const int r = r0 + u * rr.step();
+				const bool isv = r >= a.k_rounds;
+				const int head = (isv ? r - a.k_rounds : r) * rows + sub;
+				word[u] = 0;
+				scale[u] = __half();
+				if (r >= n || head >= a.p.KVH)
+					continue;
+				const uint8_t *rec = record(a.p, page, head, isv);
+				scale[u] = reinterpret_cast<const __half *>(
+					rec + ((D / 2) << a.p.page_log2))[row * nb + b];
+				word[u] = *reinterpret_cast<const uint32_t *>(rec + row * (D / 2) +
+									      row_word_at(b, nb, isv));
+			}
+#pragma unroll
+			for (int u = 0; u < kGatherBatch; u++) {
+				const int r = r0 + u * rr.step();
+				const bool isv = r >= a.k_rounds;
+				const int head = (isv ? r - a.k_rounds : r) * rows + sub;
+				uint32_t by[2];
+				row_bytes(word[u], b, isv, by);
+				if (r >= n || head >= a.p.KVH)
+					continue;
+				const float d = __half2float(scale[u]);
+				float f[8];
+#pragma unroll
+				for (int w = 0; w < 2; w++) {
+					const uint32_t x = e0 % 32 >= 16 ? by[w] >> 4 : by[w];
+#pragma unroll
+					for (int k = 0; k < 4; k++)
+						f[4 * w + k] = __fmul_rn((float)((int)(x >> (8 * k) & 15) - 8), d);
+				}
+				Raw<T, 8, VEC> x;
+				x.set(f);
+				x.store(isv ? vo + head * a.v.out_hs : ko + head * a.k.out_hs);
+			}
+		}
 	}
 }
 
-// slices of a token's items: enough CTAs for few tokens, one for many
-unsigned slices(int64_t items, int64_t n_tokens)
+int log2_of(int n)
 {
-	int64_t y = (items + kAppendThreads - 1) / kAppendThreads;
-	const int64_t fill = (4 * (int64_t)sm_count() + n_tokens - 1) / n_tokens;
-	y = y < fill ? y : fill;
-	return (unsigned)(y < 1 ? 1 : y < 65535 ? y : 65535);
+	int l = 0;
+	while (1 << l < n)
+		l++;
+	return l;
 }
 
-template <typename T, bool VEC, int LAYOUT>
-cudaError_t launch_append_as(const AppendArgs<T> &a, cudaStream_t st)
+template <typename T, bool VEC, int TURN>
+cudaError_t launch_append_as(AppendArgs<T> a, cudaStream_t st)
 {
-	constexpr int N = kVec<T>, QN = VEC ? N : LAYOUT == MOE_ROPE_PAIRS ? 2 : 1;
-	const int64_t items = (int64_t)a.q.n * RopeItem<QN, LAYOUT>::per_head(a.p.head_len, a.r.half) +
-			      31 + 2 * (int64_t)a.p.KVH * (a.p.head_len / N);
-	append_kernel<T, VEC, LAYOUT><<<dim3((unsigned)a.b.T, slices(items, a.b.T)), kAppendThreads,
-					(a.r.half ? a.r.half : 1) * sizeof(float2), st>>>(a);
+	const int D = a.p.head_len, m = 32 / (D / 8);
+	a.per_q = FastDiv(D - a.r.half);
+	a.per_log2 = log2_of(D / 8);
+	const int q_rounds = TURN == kTurnAny ? (a.q.n * (D - a.r.half) + 31) / 32 : (a.q.n + m - 1) / m;
+	const TokenSplit s = split_tokens(a.b.T, q_rounds + 2 * ((a.p.KVH + m - 1) / m), a.r.half);
+	a.cut = s;
+	a.half = FastDiv(a.r.half ? a.r.half : 1);
+	const size_t smem = (s.tokens * a.r.half) * sizeof(float2) +
+			    kAppendThreads / 32 * RowStream<T, VEC>::kWarpBytes;
+	if (cudaError_t e = ensure_smem(append_kernel<T, VEC, TURN>, smem))
+		return e;
+	append_kernel<T, VEC, TURN><<<dim3((unsigned)((a.b.T + s.tokens - 1) / s.tokens),
+					   1u << s.slices_log2), kAppendThreads, smem, st>>>(a);
 	return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t launch_append(const AppendArgs<T> &a, int layout, bool vec, cudaStream_t st)
 {
-	if (layout == MOE_ROPE_PAIRS)
-		return vec ? launch_append_as<T, true, MOE_ROPE_PAIRS>(a, st)
-			   : launch_append_as<T, false, MOE_ROPE_PAIRS>(a, st);
-	return vec && a.r.half % kVec<T> == 0 ? launch_append_as<T, true, MOE_ROPE_HALVES>(a, st)
-					      : launch_append_as<T, false, MOE_ROPE_HALVES>(a, st);
+	switch (turn_of(layout, a.r.half)) {
+	case kTurnPairs:
+		return vec ? launch_append_as<T, true, kTurnPairs>(a, st)
+			   : launch_append_as<T, false, kTurnPairs>(a, st);
+	case kTurnHalves:
+		return vec ? launch_append_as<T, true, kTurnHalves>(a, st)
+			   : launch_append_as<T, false, kTurnHalves>(a, st);
+	default:
+		return vec ? launch_append_as<T, true, kTurnAny>(a, st)
+			   : launch_append_as<T, false, kTurnAny>(a, st);
+	}
 }
 
 template <typename T>
-cudaError_t launch_gather(const GatherArgs<T> &a, bool vec, cudaStream_t st)
+cudaError_t launch_gather(GatherArgs<T> a, bool vec, cudaStream_t st)
 {
-	const int64_t items = (int64_t)(a.k.n + a.v.n) * (a.p.head_len / kVec<T>);
-	const dim3 grid((unsigned)a.b.T, slices(items, a.b.T));
+	const int m = 32 / (a.p.head_len / 8), rounds = (a.p.KVH + m - 1) / m;
+	a.per_log2 = log2_of(a.p.head_len / 8);
+	a.k_rounds = a.k.n ? rounds : 0;
+	a.v_rounds = a.v.n ? rounds : 0;
+	const TokenSplit s = split_tokens(a.b.T, a.k_rounds + a.v_rounds, 0);
+	a.cut = s;
+	const dim3 grid((unsigned)((a.b.T + s.tokens - 1) / s.tokens), 1u << s.slices_log2);
 	if (vec)
 		gather_kernel<T, true><<<grid, kAppendThreads, 0, st>>>(a);
 	else

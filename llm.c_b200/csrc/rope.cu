@@ -11,109 +11,193 @@
 #include "kv.cuh"
 
 #include <cmath>
+#include <type_traits>
 #include <vector>
 
 namespace moe {
 namespace {
 
-constexpr int kRopeThreads = 256;
-constexpr int kRopeBatch = 4;   // items of a thread whose loads are in flight together
+constexpr int kRopeThreads = 256, kRopeCtas = 4;
 
 template <typename T>
 struct RopeKernelArgs {
 	RopeArgs r;
 	const int32_t *pos;
 	Heads<T> q, k;
-	int head_len;
+	int n_tokens, head_len;
+	TokenSplit cut;
+	FastDiv half;          // pairs, to divide by
+	int per_log2;          // rope_kernel: a row's lanes
+	int rounds;            // a token's
+	FastDiv per;           // rope_any_kernel: a head's items
 	int32_t *err;
 };
 
-// grid (token, slice of its items): bound by the bytes of q and k, read once
-// and written once.  A thread's first loads leave before the position and the
-// angles, which stand two dependent loads away, are known.
-template <typename T, int N, bool VEC, int LAYOUT>
-__global__ void __launch_bounds__(kRopeThreads) rope_kernel(RopeKernelArgs<T> a)
+// the angles of the CTA's tokens, and whether their positions are in range
+template <typename T>
+__device__ __forceinline__ void token_angles(const RopeKernelArgs<T> &a, int t0, int nt, float2 *cs,
+					     int *ok)
 {
-	extern __shared__ float2 cs[];
-	const int t = blockIdx.x;
-	const int per = RopeItem<N, LAYOUT>::per_head(a.head_len, a.r.half);
-	const int nq = a.q.n * per, total = nq + a.k.n * per;
-	const int step = gridDim.y * kRopeThreads;
-	const int pos = a.pos[t];
-	bool ready = false;
-	for (int i0 = blockIdx.y * kRopeThreads + threadIdx.x; __syncthreads_or(i0 < total);
-	     i0 += kRopeBatch * step) {
-		float x[kRopeBatch][N], y[kRopeBatch][N];
-#pragma unroll
-		for (int u = 0; u < kRopeBatch; u++) {
-			const int i = i0 + u * step;
-			if (i < total) {
-				const bool isq = i < nq;
-				const Heads<T> &h = isq ? a.q : a.k;
-				const int j = isq ? i : i - nq;
-				const RopeItem<N, LAYOUT> it(j % per, a.r.half);
-				const T *p = h.in + t * h.in_ts + (j / per) * h.in_hs;
-				load_n<T, N, VEC>(p + it.e0, x[u]);
-				if (LAYOUT == MOE_ROPE_HALVES && it.e1 >= 0)
-					load_n<T, N, VEC>(p + it.e1, y[u]);
-			}
+	const int half = a.r.half;
+	for (int p = threadIdx.x; p < nt * half; p += kRopeThreads) {
+		const int t = a.half.div(p), pos = a.pos[t0 + t];
+		const bool in = pos >= 0 && pos < a.r.max_position;
+		if (p == t * half) {
+			ok[t] = in;
+			if (!in)
+				atomicOr(a.err, kKvErrPos);
 		}
-		if (!ready) {
-			if (pos < 0 || pos >= a.r.max_position) {
-				if (threadIdx.x == 0)
-					atomicOr(a.err, kKvErrPos);
-				return;   // the whole CTA: pos is the token's
-			}
-			rope_angles(a.r, pos, cs);
-			__syncthreads();
-			ready = true;
-		}
+		if (in)
+			cs[p] = rope_angle(a.r, pos, p - t * half);
+	}
+	__syncthreads();
+}
+
+// grid (token group, slice of a token's rounds): bound by the bytes of q and k, read
+// once and written once.  A lane has 8 values of a row and the same place in every
+// row it meets, so a token's angles stay in its registers.  The first loads leave
+// before the positions and their angles, two dependent loads away, are known.
+template <typename T, bool VEC, int TURN>
+__global__ void __launch_bounds__(kRopeThreads, kRopeCtas) rope_kernel(const __grid_constant__ RopeKernelArgs<T> a)
+{
+	extern __shared__ uint4 smem[];
+	__shared__ int ok[kGroupTokens];
+	uint8_t *slots = reinterpret_cast<uint8_t *>(smem);
+	float2 *cs = reinterpret_cast<float2 *>(   // [token][pair]
+		slots + kRopeThreads / 32 * RowStream<T, VEC>::kWarpBytes);
+	const int half = a.r.half, lane = threadIdx.x % 32;
+	const int t0 = blockIdx.x * a.cut.tokens, nt = min(a.cut.tokens, a.n_tokens - t0);
+	const int ml = 5 - a.per_log2;   // rows of a round, log2
+	const int e0 = (lane & ((1 << a.per_log2) - 1)) * 8, sub = lane >> a.per_log2;
+	const Rounds rr(a.cut, blockIdx.y);
+	RowStream<T, VEC> stream(slots, 1 << a.per_log2);
+	const int starts[2] = {rr.first, rr.start((a.q.n + (1 << ml) - 1) >> ml)};
+	auto reader = [&](int s, int t) {
+		const Heads<T> &h = s ? a.k : a.q;
+		return RowReader<T, VEC>(stream, h, t0 + t, t < nt ? h.n : 0, ml, sub, e0, starts[s],
+					 rr.step_log2);
+	};
+	// the first rows leave before the angles are known: of q, or of k in a warp
+	// that has none of q
+	const int early = reader(0, rr.token).w.left > 0 ? 0 : 1;
+	{
+		RowReader<T, VEC> first = early ? reader(1, rr.token) : reader(0, rr.token);
+		first.begin();
+	}
+	token_angles(a, t0, nt, cs, ok);
+	Turn8<TURN> tn(e0, half);
+	for (int t = rr.token; t < nt; t += rr.token_step) {
+		const bool good = ok[t];
+		if (good)
+			tn.angles(cs + t * half, e0, half);
 #pragma unroll
-		for (int u = 0; u < kRopeBatch; u++) {
-			const int i = i0 + u * step;
-			if (i < total) {
-				const bool isq = i < nq;
-				const Heads<T> &h = isq ? a.q : a.k;
-				const int j = isq ? i : i - nq;
-				const RopeItem<N, LAYOUT> it(j % per, a.r.half);
-				it.apply(x[u], y[u], cs, a.r.half);
-				T *p = h.out + t * h.out_ts + (j / per) * h.out_hs;
-				store_n<T, N, VEC>(p + it.e0, x[u]);
-				if (LAYOUT == MOE_ROPE_HALVES && it.e1 >= 0)
-					store_n<T, N, VEC>(p + it.e1, y[u]);
+		for (int s = 0; s < 2; s++) {
+			const Heads<T> &h = s ? a.k : a.q;
+			RowReader<T, VEC> in = reader(s, t);
+			RowWalk<T> w = in.w;
+			if (t == rr.token && s == early)
+				in.skip_begun();
+			else
+				in.begin();
+			T *out = h.out + (int64_t)(t0 + t) * h.out_ts + (int64_t)w.row * h.out_hs + e0;
+			const int64_t d = (int64_t)w.step_rows * h.out_hs;
+			for (; w.left > 0; w.left--, w.row += w.step_rows, out += d) {
+				Raw<T, 8, VEC> x;
+				stream.pop(x);
+				float f[8];
+				tn.apply(x, f);
+				if (tn.turning)   // what does not turn keeps its bits
+					x.set(f);
+				stream.store(x, good && w.has() ? out : nullptr);
+				in.next();
 			}
 		}
 	}
+	stream.finish();
 }
 
-template <typename T, int N, bool VEC, int LAYOUT>
-cudaError_t launch_rope_as(const RopeKernelArgs<T> &a, int64_t n_tokens, cudaStream_t st)
+// Rows that rope_kernel does not take: N = 2 values a thread where head_len is no
+// multiple of 8, or its vectors no power of two up to 32; PairItems (TURN kTurnAny)
+// where halves are no multiple of 8.
+template <typename T, int TURN>
+__global__ void __launch_bounds__(kRopeThreads) rope_any_kernel(const __grid_constant__ RopeKernelArgs<T> a)
 {
-	const int per = RopeItem<N, LAYOUT>::per_head(a.head_len, a.r.half);
-	const int64_t total = (int64_t)(a.q.n + a.k.n) * per;
-	// few tokens: a token's items over several CTAs, each thread one item
-	int64_t y = (total + kRopeThreads - 1) / kRopeThreads;
-	const int64_t fill = (4 * (int64_t)sm_count() + n_tokens - 1) / n_tokens;
-	y = y < fill ? y : fill;
-	y = y < 65535 ? y : 65535;
-	rope_kernel<T, N, VEC, LAYOUT>
-		<<<dim3((unsigned)n_tokens, (unsigned)y), kRopeThreads, a.r.half * sizeof(float2), st>>>(a);
-	return cudaGetLastError();
+	extern __shared__ float2 cs[];
+	__shared__ int ok[kGroupTokens];
+	const int half = a.r.half, lane = threadIdx.x % 32;
+	const int t0 = blockIdx.x * a.cut.tokens, nt = min(a.cut.tokens, a.n_tokens - t0);
+	const Rounds rr(a.cut, blockIdx.y);
+	const int nq = a.q.n * a.per.n, items = nq + a.k.n * a.per.n;
+	token_angles(a, t0, nt, cs, ok);
+	for (int t = rr.token; t < nt; t += rr.token_step) {
+		if (!ok[t])
+			continue;
+		for (int r = rr.first; r < a.rounds; r += rr.step()) {
+			int j = r * 32 + lane;
+			if (j >= items)
+				break;
+			const bool isq = j < nq;
+			const Heads<T> &h = isq ? a.q : a.k;
+			j -= isq ? 0 : nq;
+			const int head = a.per.div(j), i = j - head * a.per.n;
+			const T *in = h.in + (int64_t)(t0 + t) * h.in_ts + head * h.in_hs;
+			T *out = h.out + (int64_t)(t0 + t) * h.out_ts + head * h.out_hs;
+			if constexpr (TURN == kTurnAny) {
+				PairItem<T> x;
+				x.load(in, i, half);
+				x.turn_store(out, i, cs + t * half, half);
+			} else {
+				Raw<T, 2, false> x;
+				x.load(in + 2 * i);
+				if (i < half) {
+					float f[2];
+					x.get(f);
+					turn(f[0], f[1], cs[t * half + i]);
+					x.set(f);
+				}
+				x.store(out + 2 * i);
+			}
+		}
+	}
 }
 
 template <typename T>
-cudaError_t launch_rope(const RopeKernelArgs<T> &a, int layout, bool vec, int64_t n_tokens,
-			cudaStream_t st)
+cudaError_t launch_rope(RopeKernelArgs<T> a, int layout, bool vec, int64_t n_tokens, cudaStream_t st)
 {
-	constexpr int V = kVec<T>;
-	if (layout == MOE_ROPE_PAIRS) {
-		if (vec && a.head_len % V == 0)
-			return launch_rope_as<T, V, true, MOE_ROPE_PAIRS>(a, n_tokens, st);
-		return launch_rope_as<T, 2, false, MOE_ROPE_PAIRS>(a, n_tokens, st);
+	const int turn = turn_of(layout, a.r.half), n8 = a.head_len / 8;
+	// a row's vectors in lanes of one warp: 1, 2, 4 .. 32 of them
+	const bool rows = turn != kTurnAny && a.head_len % 8 == 0 && n8 <= 32 && 32 % n8 == 0;
+	a.n_tokens = (int)n_tokens;
+	if (rows) {
+		a.per_log2 = 0;
+		while (1 << a.per_log2 < n8)
+			a.per_log2++;
+		const int m = 32 / n8;
+		a.rounds = (a.q.n + m - 1) / m + (a.k.n + m - 1) / m;
+	} else {
+		const bool pairs = layout == MOE_ROPE_HALVES;
+		a.per = FastDiv(pairs ? a.head_len - a.r.half : a.head_len / 2);
+		a.rounds = ((a.q.n + a.k.n) * (int)a.per.n + 31) / 32;
 	}
-	if (vec && a.head_len % V == 0 && a.r.half % V == 0)
-		return launch_rope_as<T, V, true, MOE_ROPE_HALVES>(a, n_tokens, st);
-	return launch_rope_as<T, 1, false, MOE_ROPE_HALVES>(a, n_tokens, st);
+	const TokenSplit s = split_tokens(n_tokens, a.rounds, a.r.half);
+	a.cut = s;
+	a.half = FastDiv(a.r.half);
+	const dim3 grid((unsigned)((n_tokens + s.tokens - 1) / s.tokens), 1u << s.slices_log2);
+	const size_t angles = s.tokens * a.r.half * sizeof(float2);
+	auto go = [&](auto kernel, size_t slots) -> cudaError_t {
+		const size_t smem = angles + kRopeThreads / 32 * slots;
+		if (cudaError_t e = ensure_smem(kernel, smem))
+			return e;
+		kernel<<<grid, kRopeThreads, smem, st>>>(a);
+		return cudaGetLastError();
+	};
+	constexpr size_t slots = RowStream<T, true>::kWarpBytes;
+	if (!rows)
+		return layout == MOE_ROPE_HALVES ? go(rope_any_kernel<T, kTurnAny>, 0)
+						 : go(rope_any_kernel<T, kTurnPairs>, 0);
+	if (turn == kTurnPairs)
+		return vec ? go(rope_kernel<T, true, kTurnPairs>, slots) : go(rope_kernel<T, false, kTurnPairs>, 0);
+	return vec ? go(rope_kernel<T, true, kTurnHalves>, slots) : go(rope_kernel<T, false, kTurnHalves>, 0);
 }
 
 // radians a position of every pair (moe_rope_desc's definitions)
