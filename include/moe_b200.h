@@ -574,6 +574,13 @@ MOE_API int moe_model_generate(moe_model *m, const int *prompt, size_t T, int n,
  * moe_model_generate: the prompt's prefill with the first pick, and the
  * decode steps with their picks (an eos check adds a host read per step) */
 MOE_API int moe_model_timing(moe_model *m, float *prefill_ms, float *decode_ms);
+/* The type of the model's KV cache, while it is empty (after moe_model_create or
+ * moe_model_reset): MOE_F32 (the default: the reference's, whose results it
+ * matches) or MOE_Q4_0: the paged 4-bit cache of moe_kv_*, 7.1 times smaller,
+ * through moe_kv_append and moe_kv_attention in prefill and decode.  Its keys and
+ * values are rounded to 4 bits, so results differ from the reference's by that.
+ * Every buffer of the other type is freed. */
+MOE_API int moe_model_set_kv(moe_model *m, int type);
 /* empty the KV cache and reset the position (a new sequence) */
 MOE_API int moe_model_reset(moe_model *m);
 /* waits for the device; MOE_OK or the first error a kernel recorded since

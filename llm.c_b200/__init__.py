@@ -173,6 +173,7 @@ SIGNATURES = {
     "moe_model_decode": (_I, [_P, _I, _I, _P]),
     "moe_model_logits": (_I, [_P, _SZ, _P]),
     "moe_model_generate": (_I, [_P, _P, _SZ, _I, _I, _P]),
+    "moe_model_set_kv": (_I, [_P, _I]),
     "moe_model_reset": (_I, [_P]),
     "moe_model_timing": (_I, [_P, C.POINTER(C.c_float), C.POINTER(C.c_float)]),
     "moe_model_status": (_I, [_P]),
@@ -741,6 +742,10 @@ class Model:
 
     def reset(self):
         check(lib().moe_model_reset(self.h))
+
+    def set_kv(self, qtype: int):
+        """the empty KV cache's type: F32, or Q4_0 (paged, 4 bits)"""
+        check(lib().moe_model_set_kv(self.h, qtype))
 
     def timing(self):
         """(prefill ms, decode ms) of the last generate, CUDA events"""

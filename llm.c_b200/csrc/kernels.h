@@ -366,9 +366,20 @@ cudaError_t launch_attn_step(const AttnStepArgs &a, cudaStream_t st);
 // MOE_PDL=0 in the environment
 bool pdl_enabled();
 
+// the QK-norm alone, in place in the fused rows (the 4-bit cache's path): q and k
+// of each token RMS-normed over the whole vector
+cudaError_t launch_qk_norm(float *qkv, const float *q_norm, const float *k_norm, int T, int nq,
+			   int nk, float eps, cudaStream_t st);
+// kvcache.cu: rows [from, from + rows) -> [to, ..) of every layer's 4-bit pages (row r in
+// page r / page_size of its layer; the ranges do not overlap)
+cudaError_t launch_kv_move_q4(uint8_t *pages, int64_t layer_bytes, int64_t page_bytes, int L,
+			      int KVH, int HL, int page_log2, int from, int to, int rows,
+			      cudaStream_t st);
+
 // greedy pick (main.c:189-193: the first maximum) of logits [V] into
 // state[0] and picks[state[6] % pick_cap] (state[6] counts the picks); with
-// advance, the decode state {tok, pos, size, model_pos} moves one row on
+// advance, the decode state {tok, pos, size, model_pos} moves one row on, and
+// state[7] (the rows of the cache with the next step's) with it
 // (scratch: device, at least 4 KB, zero before the first call)
 cudaError_t launch_argmax_advance(const float *logits, int V, int C, int32_t *state,
 				  int32_t *picks, int pick_cap, int advance, float *scratch,

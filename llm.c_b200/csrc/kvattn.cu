@@ -61,7 +61,8 @@ struct AttnArgs {
 	int q_vec, o_vec;    // 16-byte aligned rows
 	int target;          // items wanted (0: one run a tile)
 	int64_t items;       // items that the workspace holds
-	float *part;         // [item][row][HL + 2]
+	float *part;         // [item][row][HL + 4]: sums, bias, weights' sum
+	int part_rows;       // rows of an item that can be in use
 };
 
 // one item of the batch
@@ -953,7 +954,7 @@ __global__ void __launch_bounds__(kAttnThreads, ATTN_MINB) kv_attn_kernel(AttnAr
 			}
 		}
 		if (it.runs > 1) {
-			float *pp = a.part + ((int64_t)blockIdx.x * RPT + r) * OS;
+			float *pp = a.part + ((int64_t)blockIdx.x * a.part_rows + r) * OS;
 			*reinterpret_cast<float4 *>(pp + e) = v;
 			if (e == 0)
 				*reinterpret_cast<float2 *>(pp + HL) = make_float2(b, l);
@@ -980,8 +981,8 @@ __global__ void __launch_bounds__(kAttnThreads) kv_merge_kernel(AttnArgs a)
 	if (!mine || r >= it.rows)
 		return;
 	const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-	const int64_t step = (int64_t)a.KVH * RPT * OS;   // between the runs of a tile
-	const float *pp = a.part + ((int64_t)it.first * RPT + r) * OS;
+	const int64_t step = (int64_t)a.KVH * a.part_rows * OS;   // between the runs of a tile
+	const float *pp = a.part + ((int64_t)it.first * a.part_rows + r) * OS;
 	const int s0 = warp * SIDE + lane / W, e = lane % W * 4;
 	constexpr int ds = kAttnWarps * SIDE;
 	float4 x[BATCH][NV];
@@ -1085,13 +1086,16 @@ Plan plan_of(const moe_kv_cache *c, const moe_kv_batch *b, int64_t H, bool fp32)
 	while (want < wave / 2)
 		want += wave;
 	p.target = (int)want;
-	p.split = p.tiles < 4 * wave;
+	// split unless there are tiles enough, or every sequence is a single run
+	const int64_t longest = (b->max_kv + kAttnTile - 1) / kAttnTile;
+	p.split = p.tiles < 4 * wave && longest > kRunMin;
 	p.items = p.tiles;
 	if (p.split) {
-		const int64_t longest = (b->max_kv + kAttnTile - 1) / kAttnTile;
 		const int64_t capped = p.tiles * longest / kRunMax + 1;
+		const int64_t most = p.tiles * ((longest + kRunMin - 1) / kRunMin);
 		p.items += 1 + (capped > p.target ? capped : p.target);
-		p.part_bytes = (size_t)(p.items * p.rpt * (HL + 4) * 4);
+		p.items = p.items < most ? p.items : most;
+		p.part_bytes = (size_t)(p.items * p.rows * (HL + 4) * 4);
 	}
 	return p;
 }
@@ -1234,6 +1238,7 @@ int moe_kv_attention(moe_kv_cache *cache, const moe_kv_batch *batch, const moe_r
 	a.target = p.split ? p.target : 0;
 	a.items = p.items;
 	a.part = static_cast<float *>(workspace);
+	a.part_rows = p.rows;
 	KV_CK(what, q->type == MOE_F32   ? launch_attn<float>(a, p, (int)D, st)
 		    : q->type == MOE_F16 ? launch_attn<__half>(a, p, (int)D, st)
 					 : launch_attn<__nv_bfloat16>(a, p, (int)D, st));

@@ -436,6 +436,26 @@ cudaError_t launch_gather(GatherArgs<T> a, bool vec, cudaStream_t st)
 	return cudaGetLastError();
 }
 
+// grid (rows, KV heads, layers x K and V): a row's codes in 8-byte words, its scales in
+// 2-byte ones
+__global__ void kv_move_q4_kernel(uint8_t *pages, int64_t layer_bytes, int64_t page_bytes, int HL,
+				  int page_log2, int from, int to)
+{
+	const int64_t half = (int64_t)(HL / 2 + HL / 16) << page_log2;
+	uint8_t *base = pages + (blockIdx.z / 2) * layer_bytes + (2 * blockIdx.y + blockIdx.z % 2) * half;
+	auto at = [&](int r) { return base + (r >> page_log2) * page_bytes; };
+	const int src = from + blockIdx.x, dst = to + blockIdx.x, mask = (1 << page_log2) - 1;
+	const int words = HL / 16, scales = HL / 32;   // of a row
+	const int sc = (HL / 2) << page_log2;
+	if ((int)threadIdx.x < words)
+		reinterpret_cast<uint64_t *>(at(dst) + (dst & mask) * (HL / 2))[threadIdx.x] =
+			reinterpret_cast<const uint64_t *>(at(src) + (src & mask) * (HL / 2))[threadIdx.x];
+	else if ((int)threadIdx.x < words + scales)
+		reinterpret_cast<uint16_t *>(at(dst) + sc + (dst & mask) * scales * 2)[threadIdx.x - words] =
+			reinterpret_cast<const uint16_t *>(at(src) + sc +
+							   (src & mask) * scales * 2)[threadIdx.x - words];
+}
+
 int page_log2_of(int64_t page_size)
 {
 	for (int i = 4; i <= 8; i++)
@@ -445,6 +465,18 @@ int page_log2_of(int64_t page_size)
 }
 
 }  // namespace
+
+cudaError_t launch_kv_move_q4(uint8_t *pages, int64_t layer_bytes, int64_t page_bytes, int L,
+			      int KVH, int HL, int page_log2, int from, int to, int rows,
+			      cudaStream_t st)
+{
+	if (rows <= 0 || from == to)
+		return cudaSuccess;
+	kv_move_q4_kernel<<<dim3(rows, KVH, 2 * L), 32, 0, st>>>(pages, layer_bytes, page_bytes, HL,
+								  page_log2, from, to);
+	return cudaGetLastError();
+}
+
 }  // namespace moe
 
 using namespace moe;

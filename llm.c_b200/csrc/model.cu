@@ -229,6 +229,22 @@ __global__ void __launch_bounds__(kNormThreads) qk_rope_kernel(QkvArgs a)
 	}
 }
 
+// grid (token, q or k): x = (x / rms) * weight in place, as qk_rope_kernel's norm
+__global__ void __launch_bounds__(kNormThreads)
+qk_norm_kernel(float *qkv, const float *q_norm, const float *k_norm, int nq, int nk, float eps)
+{
+	__shared__ float red[32];
+	const int isk = blockIdx.y, n = isk ? nk : nq;
+	float *x = qkv + (int64_t)blockIdx.x * (nq + 2 * nk) + (isk ? nq : 0);
+	const float *w = isk ? k_norm : q_norm;
+	float s = 0.0f;
+	for (int j = threadIdx.x; j < n; j += blockDim.x)
+		s = fmaf(x[j], x[j], s);
+	const float rms = sqrtf(block_sum(s, red) / (float)n + eps);
+	for (int j = threadIdx.x; j < n; j += blockDim.x)
+		x[j] = (x[j] / rms) * w[j];
+}
+
 // ---------------------------------------------------------------- attention
 constexpr int kDecThreads = 128;   // 4 warps; head_len 128: 4 elements a lane
 
@@ -750,6 +766,7 @@ argmax_advance_kernel(const float *logits, int V, int C, int32_t *state, int32_t
 			state[2] = size;
 			state[3] = mpos;
 			state[1] = mpos >= C ? size : mpos;
+			state[7] = size + 1;
 		}
 	}
 }
@@ -818,6 +835,15 @@ cudaError_t launch_qk_rope(const QkvArgs &a, cudaStream_t st)
 	if (a.HL % 2 || a.KVH <= 0 || a.H % a.KVH)
 		return cudaErrorInvalidValue;
 	qk_rope_kernel<<<dim3(a.T, 3), kNormThreads, 0, st>>>(a);
+	return cudaGetLastError();
+}
+
+cudaError_t launch_qk_norm(float *qkv, const float *q_norm, const float *k_norm, int T, int nq,
+			   int nk, float eps, cudaStream_t st)
+{
+	if (T <= 0)
+		return cudaSuccess;
+	qk_norm_kernel<<<dim3(T, 2), kNormThreads, 0, st>>>(qkv, q_norm, k_norm, nq, nk, eps);
 	return cudaGetLastError();
 }
 
@@ -915,6 +941,7 @@ cudaError_t launch_kv_shift(float *kc, float *vc, int L, int KVH, int C, int HL,
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <new>
 #include <utility>
 #include <vector>
 
@@ -959,7 +986,11 @@ int64_t row_bytes_of(int type, int64_t cols)
 // device state words
 // S_ERR: bits 1 (token id) and 2 (position / cache row) of this file's
 // kernels; S_PERR: the projections' bounded waits; S_STEP: picks made
-enum { S_TOK = 0, S_POS = 1, S_SIZE = 2, S_MPOS = 3, S_ERR = 4, S_PERR = 5, S_STEP = 6, S_WORDS = 8 };
+// S_KV: cache rows with the call's own (4-bit cache: kv_len); S_QS: q_start of a
+// prefill (0, T), S_Q1: of a decode step (0, 1)
+enum { S_TOK = 0, S_POS = 1, S_SIZE = 2, S_MPOS = 3, S_ERR = 4, S_PERR = 5, S_STEP = 6, S_KV = 7,
+       S_QS = 8, S_Q1 = 10, S_WORDS = 12 };
+constexpr int64_t kKvPage = 64;   // rows of a page of the 4-bit cache
 
 }  // namespace
 
@@ -989,7 +1020,15 @@ struct moe_model {
 	};
 	std::vector<Layer> layers;
 	float2 *rope = nullptr;          // [C][HL/2]
-	float *kc = nullptr, *vc = nullptr;  // [L][KVH][C][HL]
+	float *kc = nullptr, *vc = nullptr;  // [L][KVH][C][HL]; NULL with a 4-bit cache
+	// the 4-bit cache: every layer's pages, one behind the other
+	int kv_type = MOE_F32;
+	uint8_t *kvq = nullptr;
+	std::vector<moe_kv_cache *> kvl;
+	moe_rope *kv_rope = nullptr;
+	int32_t *kv_table = nullptr;     // page r / kKvPage holds row r
+	void *kv_ws1 = nullptr, *kv_ws = nullptr;   // attention workspaces: decode, prefill
+	size_t kv_ws1_bytes = 0, kv_ws_bytes = 0;
 	// activations (capacity cap rows)
 	int64_t cap = 0;
 	float *hidden = nullptr, *xn = nullptr, *qkv = nullptr, *q = nullptr, *att = nullptr,
@@ -1029,6 +1068,17 @@ int dalloc(moe_model *m, void **p, size_t bytes)
 	m->owned.push_back(*p);
 	m->bytes += bytes;
 	return MOE_OK;
+}
+
+void dfree(moe_model *m, void *p, size_t bytes)
+{
+	for (size_t i = 0; i < m->owned.size(); i++)
+		if (m->owned[i] == p) {
+			m->owned.erase(m->owned.begin() + (ptrdiff_t)i);
+			m->bytes -= bytes;
+			cudaFree(p);
+			return;
+		}
 }
 
 const void *host_ptr(const moe_tensor_t *t)
@@ -1121,6 +1171,59 @@ int ensure_act(moe_model *m, int64_t T)
 
 namespace {
 
+int64_t kv_pages(const moe_model *m) { return (m->C + kKvPage - 1) / kKvPage; }
+
+moe_kv_batch kv_batch(const moe_model *m, int64_t T)
+{
+	moe_kv_batch b{};
+	b.n_seqs = 1;
+	b.n_tokens = T;
+	b.max_q = T;
+	b.max_kv = m->C;
+	b.q_start = m->state + (T == 1 ? S_Q1 : S_QS);
+	b.kv_len = m->state + S_KV;
+	b.page_table = m->kv_table;
+	b.table_stride = kv_pages(m);
+	return b;
+}
+
+// QK-norm, RoPE, cache rows and attention of layer l's fused rows over the 4-bit cache
+int kv_attention(moe_model *m, int64_t l, int64_t T, const int32_t *pos_d)
+{
+	const moe_model::Layer &ly = m->layers[l];
+	const moe_kv_batch b = kv_batch(m, T);
+	if (ly.q_norm)
+		MCK(moe::launch_qk_norm(m->qkv, ly.q_norm, ly.k_norm, (int)T, (int)m->nq, (int)m->nk, 1e-5f,
+					m->st));
+	const int64_t ts = m->nq + 2 * m->nk;
+	const moe_rows q{m->qkv, MOE_F32, m->H, ts, m->HL}, k{m->qkv + m->nq, MOE_F32, m->KVH, ts, m->HL},
+		v{m->qkv + m->nq + m->nk, MOE_F32, m->KVH, ts, m->HL};
+	const moe_rows qo{m->q, MOE_F32, m->H, m->nq, m->HL}, out{m->att, MOE_F32, m->H, m->nq, m->HL};
+	MRC(moe_kv_append(m->kvl[l], &b, m->kv_rope, pos_d, &k, &v, &q, &qo, m->st));
+	const bool one = T == 1;
+	return moe_kv_attention(m->kvl[l], &b, &qo, &out, nullptr, 1.0f / m->scale_div, 1, 0,
+				one ? m->kv_ws1 : m->kv_ws, one ? m->kv_ws1_bytes : m->kv_ws_bytes, m->st);
+}
+
+// the prefill's workspace (the decode step's is its own: a graph holds it)
+int ensure_kv_ws(moe_model *m, int64_t T)
+{
+	if (m->kv_type != MOE_Q4_0 || T == 1)
+		return MOE_OK;
+	const moe_kv_batch b = kv_batch(m, T);
+	const int64_t need = moe_kv_attention_workspace(m->kvl[0], &b, m->H);
+	if (need < 0)
+		return (int)need;
+	if ((size_t)need <= m->kv_ws_bytes)
+		return MOE_OK;
+	MCK(cudaStreamSynchronize(m->st));
+	dfree(m, m->kv_ws, m->kv_ws_bytes);
+	m->kv_ws_bytes = 0;
+	MRC(dalloc(m, &m->kv_ws, (size_t)need));
+	m->kv_ws_bytes = (size_t)need;
+	return MOE_OK;
+}
+
 // The decode step (T = 1) through the fused kernels, each launched as a
 // programmatic dependent of the one before: per layer the QKV GEMV takes the
 // residual add and attn_norm into its prologue (the residual stream moves
@@ -1166,7 +1269,10 @@ int forward_step(moe_model *m, const int32_t *tok_d, const int32_t *pos_d)
 		a.eps = eps;
 		a.scale_div = m->scale_div;
 		a.err = err;
-		MCK(moe::launch_attn_step(a, m->st));
+		if (m->kv_type == MOE_Q4_0)
+			MRC(kv_attention(m, l, 1, pos_d));
+		else
+			MCK(moe::launch_attn_step(a, m->st));
 		MCK(moe::launch_gemv1(ly.wo, ly.o_t, E, m->nq, m->att, m->proj, perr, m->st, pdl));
 		MCK(moe::launch_add_norm(R, m->proj, ly.ffn_norm, 1, E, eps, m->xn, m->st, pdl));
 		MRC(moe_layer_forward(ly.moe, m->xn, m->ffn, 1, m->renorm ? MOE_RENORM : 0, m->st));
@@ -1210,9 +1316,14 @@ int forward(moe_model *m, int64_t T, const int32_t *tok_d, const int32_t *pos_d)
 		a.C = (int)m->C;
 		a.eps = eps;
 		a.err = err;
-		MCK(moe::launch_qk_rope(a, m->st));
-		MCK(moe::launch_attention(m->q, a.kc, a.vc, size_d, (int)T, (int)m->H, (int)m->KVH,
-					  (int)m->HL, (int)m->C, m->scale_div, m->part, m->att, m->st));
+		if (m->kv_type == MOE_Q4_0) {
+			MRC(kv_attention(m, l, T, pos_d));
+		} else {
+			MCK(moe::launch_qk_rope(a, m->st));
+			MCK(moe::launch_attention(m->q, a.kc, a.vc, size_d, (int)T, (int)m->H, (int)m->KVH,
+						  (int)m->HL, (int)m->C, m->scale_div, m->part, m->att,
+						  m->st));
+		}
 		MRC(moe::dense_forward(m->ds, ly.wo, ly.o_t, E, m->nq, m->att, T, m->proj, perr, m->st));
 		MCK(moe::launch_add_norm(m->hidden, m->proj, ly.ffn_norm, (int)T, E, eps, m->xn, m->st));
 		MRC(moe_layer_forward(ly.moe, m->xn, m->ffn, T, m->renorm ? MOE_RENORM : 0, m->st));
@@ -1223,8 +1334,8 @@ int forward(moe_model *m, int64_t T, const int32_t *tok_d, const int32_t *pos_d)
 }
 
 // the host's cache size and position into the device state (S_POS, S_SIZE,
-// S_MPOS; S_TOK too when tok >= 0)
-int write_state(moe_model *m, int64_t pos, int tok)
+// S_MPOS; S_TOK too when tok >= 0), and the words of a call of T tokens
+int write_state(moe_model *m, int64_t pos, int tok, int64_t T)
 {
 	m->hstate[S_TOK] = tok;
 	m->hstate[S_POS] = (int32_t)pos;
@@ -1236,6 +1347,13 @@ int write_state(moe_model *m, int64_t pos, int tok)
 	else
 		MCK(cudaMemcpyAsync(m->state + S_POS, m->hstate + S_POS, 3 * sizeof(int32_t),
 				    cudaMemcpyHostToDevice, m->st));
+	m->hstate[S_KV] = (int32_t)(m->size + T);
+	m->hstate[S_QS] = 0;
+	m->hstate[S_QS + 1] = (int32_t)T;
+	m->hstate[S_Q1] = 0;
+	m->hstate[S_Q1 + 1] = 1;
+	MCK(cudaMemcpyAsync(m->state + S_KV, m->hstate + S_KV, (S_WORDS - S_KV) * sizeof(int32_t),
+			    cudaMemcpyHostToDevice, m->st));
 	// the pinned words may be rewritten by the next call before this copy ran
 	MCK(cudaStreamSynchronize(m->st));
 	return MOE_OK;
@@ -1246,6 +1364,15 @@ int rotate(moe_model *m)
 {
 	const int64_t keep = std::min<int64_t>(m->C / 2, m->size);
 	const int64_t drop = m->size - keep;
+	if (m->kv_type == MOE_Q4_0) {
+		const int64_t pb = (int64_t)moe_kv_page_bytes(kKvPage, m->KVH, m->HL, MOE_Q4_0);
+		for (int64_t done = 0; drop > 0 && done < keep; done += drop)
+			MCK(moe::launch_kv_move_q4(m->kvq, kv_pages(m) * pb, pb, (int)m->L, (int)m->KVH,
+						   (int)m->HL, 6, (int)(drop + done), (int)done,
+						   (int)std::min(drop, keep - done), m->st));
+		m->size = keep;
+		return MOE_OK;
+	}
 	MCK(moe::launch_kv_shift(m->kc, m->vc, (int)m->L, (int)m->KVH, (int)m->C, (int)m->HL,
 				 (int)keep, (int)drop, m->st));
 	m->size = keep;
@@ -1329,9 +1456,94 @@ int take_state_error(moe_model *m)
 		return mfail(MOE_ERR_INVALID, "moe_model: %s%s", (e[0] & 1) ? "token id outside the "
 			     "vocabulary; " : "", (e[0] & 2) ? "position or cache row out of range" : "");
 	}
+	// every layer's cache meets the same lengths, pages and positions
+	if (!m->kvl.empty())
+		MRC(moe_kv_status(m->kvl[0]));
 	for (const auto &ly : m->layers)
 		if (ly.moe)
 			MRC(moe_layer_status(ly.moe));
+	return MOE_OK;
+}
+
+void free_kv(moe_model *m)
+{
+	for (moe_kv_cache *c : m->kvl)
+		moe_kv_destroy(c);
+	m->kvl.clear();
+	moe_rope_destroy(m->kv_rope);
+	m->kv_rope = nullptr;
+}
+
+size_t kv_f32_bytes(const moe_model *m) { return (size_t)(m->L * m->KVH * m->C * m->HL) * 4; }
+
+// the cache of type `type` instead of the present one, both empty
+int change_kv(moe_model *m, int type)
+{
+	const int64_t n = kv_pages(m);
+	const int64_t pb = (int64_t)moe_kv_page_bytes(kKvPage, m->KVH, m->HL, MOE_Q4_0);
+	void *v;
+	if (type == MOE_F32) {
+		const size_t cache = kv_f32_bytes(m);
+		if (!m->kc) {
+			MRC(dalloc(m, &v, cache));
+			m->kc = static_cast<float *>(v);
+		}
+		if (!m->vc) {
+			MRC(dalloc(m, &v, cache));
+			m->vc = static_cast<float *>(v);
+		}
+		free_kv(m);
+		dfree(m, m->kvq, (size_t)(m->L * n * pb));
+		dfree(m, m->kv_table, (size_t)n * 4);
+		dfree(m, m->kv_ws1, m->kv_ws1_bytes);
+		dfree(m, m->kv_ws, m->kv_ws_bytes);
+		m->kvq = nullptr;
+		m->kv_table = nullptr;
+		m->kv_ws1 = m->kv_ws = nullptr;
+		m->kv_ws1_bytes = m->kv_ws_bytes = 0;
+		m->kv_type = type;
+		return MOE_OK;
+	}
+	if (!m->kvq) {
+		MRC(dalloc(m, &v, (size_t)(m->L * n * pb)));
+		m->kvq = static_cast<uint8_t *>(v);
+		MCK(cudaMemset(v, 0, (size_t)(m->L * n * pb)));
+	}
+	if (!m->kv_table) {
+		std::vector<int32_t> table((size_t)n);
+		for (int64_t i = 0; i < n; i++)
+			table[(size_t)i] = (int32_t)i;
+		MRC(dalloc(m, &v, (size_t)n * 4));
+		m->kv_table = static_cast<int32_t *>(v);
+		MCK(cudaMemcpy(v, table.data(), (size_t)n * 4, cudaMemcpyHostToDevice));
+	}
+	if (!m->kv_rope) {
+		moe_rope_desc r{};
+		r.rot = m->HL;
+		r.max_position = m->C;
+		r.layout = MOE_ROPE_PAIRS;
+		r.theta = m->d.rope_theta;
+		MRC(moe_rope_create(&m->kv_rope, &r));
+	}
+	while ((int64_t)m->kvl.size() < m->L) {
+		const int64_t l = (int64_t)m->kvl.size();
+		moe_kv_desc d{n, kKvPage, m->KVH, m->HL, MOE_Q4_0, m->kvq + l * n * pb};
+		moe_kv_cache *c;
+		MRC(moe_kv_create(&c, &d));
+		m->kvl.push_back(c);
+	}
+	if (!m->kv_ws1) {
+		const moe_kv_batch b = kv_batch(m, 1);
+		const int64_t need = moe_kv_attention_workspace(m->kvl[0], &b, m->H);
+		if (need < 0)
+			return (int)need;
+		MRC(dalloc(m, &m->kv_ws1, (size_t)need));
+		m->kv_ws1_bytes = (size_t)need;
+	}
+	dfree(m, m->kc, kv_f32_bytes(m));
+	dfree(m, m->vc, kv_f32_bytes(m));
+	m->kc = m->vc = nullptr;
+	m->kv_type = type;
 	return MOE_OK;
 }
 
@@ -1475,6 +1687,7 @@ void free_model(moe_model *m)
 	if (m->st)
 		cudaStreamSynchronize(m->st);
 	drop_graph(m);
+	free_kv(m);
 	for (auto &ly : m->layers)
 		if (ly.moe)
 			moe_layer_destroy(ly.moe);
@@ -1505,7 +1718,8 @@ int prefill_impl(moe_model *m, const int *tok, const int *pos, int64_t T)
 	if (T > m->cap)
 		drop_graph(m);   // the graph holds the activation pointers
 	MRC(ensure_act(m, T));
-	MRC(write_state(m, 0, -1));
+	MRC(ensure_kv_ws(m, T));
+	MRC(write_state(m, 0, -1, T));
 	MCK(cudaMemcpyAsync(m->tok, tok, (size_t)T * 4, cudaMemcpyHostToDevice, m->st));
 	MCK(cudaMemcpyAsync(m->pos, pos, (size_t)T * 4, cudaMemcpyHostToDevice, m->st));
 	MRC(forward(m, T, m->tok, m->pos));
@@ -1535,7 +1749,7 @@ int decode_impl(moe_model *m, int tok, int64_t pos, bool host_tok, bool sync_sta
 		return mfail(MOE_ERR_INVALID, "moe_model_decode: position %lld", (long long)pos);
 	MRC(ensure_act(m, 1));
 	if (host_tok || sync_state || rotated)
-		MRC(write_state(m, pos, host_tok ? tok : -1));
+		MRC(write_state(m, pos, host_tok ? tok : -1, 1));
 	if (m->graphable)
 		MRC(capture(m));
 	if (m->gexec)
@@ -1546,6 +1760,21 @@ int decode_impl(moe_model *m, int tok, int64_t pos, bool host_tok, bool sync_sta
 	m->mpos += 1;
 	m->last_T = 1;
 	m->logits_row = 0;
+	return MOE_OK;
+}
+
+// one eager decode step on token 0 into the empty cache: every layer's
+// one-row scratch and every kernel attribute exist before a capture
+int warm_up(moe_model *m)
+{
+	MRC(ensure_act(m, 1));
+	MRC(write_state(m, 0, 0, 1));
+	MRC(decode_step_body(m));
+	const cudaError_t e = cudaStreamSynchronize(m->st);
+	if (e != cudaSuccess)
+		return mcuda(e, "moe_model: warm-up");
+	MRC(take_state_error(m));
+	MCK(cudaMemset(m->state, 0, S_WORDS * 4));
 	return MOE_OK;
 }
 
@@ -1678,22 +1907,7 @@ int moe_model_create(moe_model **out, const moe_model_desc *desc)
 			return rc;
 		}
 	}
-	// one eager decode step on token 0 into the empty cache: every layer's
-	// one-row scratch and every kernel attribute exist before a capture
-	rc = ensure_act(m, 1);
-	if (rc == MOE_OK)
-		rc = write_state(m, 0, 0);
-	if (rc == MOE_OK)
-		rc = decode_step_body(m);
-	if (rc == MOE_OK) {
-		const cudaError_t e = cudaStreamSynchronize(m->st);
-		rc = e == cudaSuccess ? take_state_error(m) : mcuda(e, "moe_model_create: warm-up");
-	}
-	if (rc == MOE_OK) {
-		const cudaError_t e = cudaMemset(m->state, 0, S_WORDS * 4);
-		if (e != cudaSuccess)
-			rc = mcuda(e, "moe_model_create: state");
-	}
+	rc = warm_up(m);
 	if (rc != MOE_OK) {
 		free_model(m);
 		return rc;
@@ -1717,6 +1931,27 @@ int moe_model_reset(moe_model *m)
 	m->last_T = 0;
 	m->logits_row = -1;
 	return MOE_OK;
+}
+
+int moe_model_set_kv(moe_model *m, int type)
+{
+	if (!m)
+		return mfail(MOE_ERR_INVALID, "moe_model_set_kv: null model");
+	if (type != MOE_F32 && type != MOE_Q4_0)
+		return mfail(MOE_ERR_UNSUPPORTED, "moe_model_set_kv: type %d (MOE_F32 or MOE_Q4_0)", type);
+	if (m->size != 0)
+		return mfail(MOE_ERR_INVALID, "moe_model_set_kv: the cache holds %lld rows",
+			     (long long)m->size);
+	if (type == m->kv_type)
+		return MOE_OK;
+	MCK(cudaStreamSynchronize(m->st));
+	drop_graph(m);
+	try {
+		MRC(change_kv(m, type));
+	} catch (const std::bad_alloc &) {
+		return mfail(MOE_ERR_NOMEM, "moe_model_set_kv: host memory");
+	}
+	return warm_up(m);
 }
 
 int moe_model_prefill(moe_model *m, const int *tok, const int *pos, size_t T, float *output)
