@@ -99,63 +99,54 @@ __device__ __forceinline__ int seq_tiles(const AttnArgs &a, int n, int kv)
 	return (kv + kAttnTile - 1) / kAttnTile - lo / kAttnTile;
 }
 
-__device__ __forceinline__ int64_t warp_sum64(int64_t v)
-{
-#pragma unroll
-	for (int o = 16; o; o /= 2)
-		v += __shfl_xor_sync(0xffffffffu, v, o);
-	return v;
-}
-
 // sums of v over the lanes up to this one
-__device__ __forceinline__ int64_t warp_scan64(int64_t v)
+__device__ __forceinline__ int warp_scan(int v)
 {
 	const int lane = threadIdx.x % 32;
 #pragma unroll
 	for (int o = 1; o < 32; o *= 2) {
-		const int64_t w = __shfl_up_sync(0xffffffffu, v, o);
+		const int w = __shfl_up_sync(0xffffffffu, v, o);
 		v += lane >= o ? w : 0;
 	}
 	return v;
 }
 
-// Item `index` of the batch (ITEM), or tile `index` of its query tiles with
-// the tile's number of runs.  Every warp of both kernels derives the same plan
-// from the lengths, 32 sequences at a time: all work in key tiles over the
-// items wanted gives the run's length; sums over the sequences before give a
-// sequence's first item.
+// Item `index` of the batch (ITEM), or tile `index` of its query tiles with the
+// tile's number of runs, by one warp.  Every CTA of both kernels derives the same
+// plan from the lengths, 32 sequences at a time: all work in key tiles over the
+// items wanted gives the run's length (in fp32: any length is right); sums over the
+// sequences before give a sequence's first item.  The sums fit 32 bits where the
+// arrays keep to the call's bounds (the host checks those).
 template <int RPT, bool ITEM>
-__device__ __forceinline__ bool find_item(const AttnArgs &a, int64_t index, Item &f)
+__device__ __forceinline__ bool find_item(const AttnArgs &a, int index, Item &f)
 {
 	const int lane = threadIdx.x % 32, B = a.b.B;
 	int s0 = 0, n = 0, kv = 0;
-	int64_t run = (int64_t)1 << 40;   // target 0: query tiles enough, one run each
+	int run = 1 << 30;   // target 0: query tiles enough, one run each
 	if (a.target) {
-		int64_t all = 0;
+		float all = 0.0f;
 		for (int b = lane; b < B; b += 32)
 			if (seq_of(a, b, s0, n, kv))
-				all += (int64_t)((n * a.G + RPT - 1) / RPT) * seq_tiles(a, n, kv);
-		all = warp_sum64(all) * a.KVH;
-		run = (int64_t)ceilf((float)all / a.target);   // about so: any run is right
-		run = run < kRunMin ? kRunMin : run > kRunMax ? kRunMax : run;
+				all += (float)((n * a.G + RPT - 1) / RPT) * (float)seq_tiles(a, n, kv);
+		run = (int)fminf(ceilf(warp_sum(all) * a.KVH / a.target), (float)kRunMax);
+		run = max(run, kRunMin);
 	}
-	int64_t item0 = 0, tile0 = 0;
+	int item0 = 0, tile0 = 0;
 	for (int b0 = 0; b0 < B; b0 += 32) {
 		const int b = b0 + lane;
-		int64_t tiles = 0, runs = 0;
+		int tiles = 0, runs = 0;
 		if (B > 32 || !a.target) {
 			n = 0;
 			if (b < B)
 				seq_of(a, b, s0, n, kv);
 		}
 		if (b < B && n > 0) {
-			const unsigned step = (unsigned)min(run, (int64_t)1 << 30);
-			tiles = (n * a.G + RPT - 1) / RPT;   // the host keeps n G to 2^30
-			runs = max(1u, (seq_tiles(a, n, kv) + step - 1) / step);
+			tiles = (n * a.G + RPT - 1) / RPT;
+			runs = max(1, (int)((unsigned)(seq_tiles(a, n, kv) + run - 1) / (unsigned)run));
 		}
-		const int64_t items = tiles * runs * a.KVH;
-		const int64_t iend = item0 + warp_scan64(items);
-		const int64_t tend = ITEM ? iend : tile0 + warp_scan64(tiles * a.KVH);
+		const int items = tiles * runs * a.KVH;
+		const int iend = item0 + warp_scan(items);
+		const int tend = ITEM ? iend : tile0 + warp_scan(tiles * a.KVH);
 		const unsigned m = __ballot_sync(0xffffffffu, index < (ITEM ? iend : tend));
 		if (m) {
 			// the first sequence that ends behind it
@@ -165,39 +156,57 @@ __device__ __forceinline__ bool find_item(const AttnArgs &a, int64_t index, Item
 			kv = __shfl_sync(0xffffffffu, kv, src);
 			tiles = __shfl_sync(0xffffffffu, tiles, src);
 			runs = __shfl_sync(0xffffffffu, runs, src);
-			const int64_t i0 = __shfl_sync(0xffffffffu, iend - items, src);
-			const int64_t t0 = __shfl_sync(0xffffffffu, tend - tiles * a.KVH, src);
-			const int64_t at = index - (ITEM ? i0 : t0);
+			const int i0 = __shfl_sync(0xffffffffu, iend - items, src);
+			const int t0 = __shfl_sync(0xffffffffu, tend - tiles * a.KVH, src);
+			const unsigned at = index - (ITEM ? i0 : t0);
 			// KV heads side by side; the last tiles, which see the most, first
 			f.b = b0 + src;
 			f.s0 = s0;
 			f.n = n;
 			f.kv = kv;
-			const unsigned rest = (unsigned)at / a.KVH;   // at is below 2^31, as the grid
-			f.kvh = (unsigned)at - rest * a.KVH;
+			const unsigned rest = at / (unsigned)a.KVH;
+			f.kvh = at - rest * a.KVH;
 			const unsigned rank = ITEM ? rest / (unsigned)runs : rest;
 			f.run = ITEM ? rest - rank * (unsigned)runs : 0;
-			const int64_t first = i0 + rank * runs * a.KVH + f.kvh;
-			f.first = (int)first;
-			f.tile = (int)(tiles - 1 - rank);
+			f.first = i0 + rank * runs * a.KVH + f.kvh;
+			f.tile = tiles - 1 - (int)rank;
 			f.r0 = f.tile * RPT;
 			f.rows = min(RPT, n * a.G - f.r0);
 			const int p0 = kv - n + f.r0 / a.G, p1 = kv - n + (f.r0 + f.rows - 1) / a.G;
 			f.lo = a.window ? max(0, p0 - a.window + 1) : 0;
 			f.hi = a.causal ? min(kv, p1 + 1) : kv;
 			const int ta = f.lo / kAttnTile, tb = max(ta, (f.hi + kAttnTile - 1) / kAttnTile);
-			const unsigned step = (unsigned)min(run, (int64_t)1 << 30);
-			f.runs = max(1u, (tb - ta + step - 1) / step);
-			f.t0 = (int)min((int64_t)tb, ta + f.run * run);
-			f.t1 = (int)min((int64_t)tb, f.t0 + run);
+			f.runs = max(1, (int)((unsigned)(tb - ta + run - 1) / (unsigned)run));
+			f.t0 = min(tb, ta + f.run * run);
+			f.t1 = min(tb, f.t0 + run);
 			// q_start that does not rise can name more items than it has
 			// tokens for: those behind the plan's bound are left out
-			return first + (runs - 1) * a.KVH < a.items && (!ITEM || f.run < f.runs);
+			return f.first >= 0 && f.first + (int64_t)(runs - 1) * a.KVH < a.items &&
+			       (!ITEM || f.run < f.runs);
 		}
 		item0 = __shfl_sync(0xffffffffu, iend, 31);
 		tile0 = __shfl_sync(0xffffffffu, tend, 31);
 	}
 	return false;
+}
+
+// found by the CTA's first warp for all of them
+template <int RPT, bool ITEM>
+__device__ __forceinline__ bool cta_item(const AttnArgs &a, int index, Item &f)
+{
+	__shared__ Item found;
+	__shared__ int ok;
+	if (threadIdx.x < 32) {
+		Item x;
+		const bool in = find_item<RPT, ITEM>(a, index, x);
+		if (threadIdx.x == 0) {
+			found = x;
+			ok = in;
+		}
+	}
+	__syncthreads();
+	f = found;
+	return ok;
 }
 
 __device__ __forceinline__ void mma_step(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -401,7 +410,7 @@ __global__ void __launch_bounds__(kAttnThreads, ATTN_MINB) kv_attn_kernel(AttnAr
 
 	griddep_launch_dependents();
 	Item it;
-	if (!find_item<RPT, true>(a, blockIdx.x, it))   // the same for every warp
+	if (!cta_item<RPT, true>(a, blockIdx.x, it))
 		return;
 
 	// ---- the warp's key tiles: t0 + warp, + 4, ..: lane l keeps the pages of
@@ -441,10 +450,31 @@ __global__ void __launch_bounds__(kAttnThreads, ATTN_MINB) kv_attn_kernel(AttnAr
 	// and V's side by side over the lanes
 	constexpr int CH = SL::kCodes / 512, SLN = SL::kScales / 16, SCH = (2 * SLN + 31) / 32;
 	const uint32_t ring_at = smem_addr(ring) + lane * 16;
+	const uint8_t *codes_at = head_pages + lane * 16;
+	const uint8_t *scales_at = head_pages + ((HL / 2) << a.b.page_log2) +
+				   (lane < SLN ? lane * 16 : half_rec + (lane - SLN) * 16);
+	const uint32_t to_scales = smem_addr(ring) + (lane < SLN ? SL::kKS + lane * 16
+								 : SL::kVS + (lane - SLN) * 16);
 	unsigned ring_have = 0;   // 2 bits a stage: the halves in it
 	auto issue = [&](int i, int stage) {
 		const int k0 = key0(i);
 		const int pa = __shfl_sync(0xffffffffu, page_a, i & 31);
+		if (!small && SCH == 1 && k0 >= it.lo && k0 + 16 < it.hi && pa >= 0) {
+			// both halves, of one page
+			const int r = k0 & (P - 1);
+			const int64_t at = pa * a.page_bytes;
+			const uint8_t *p = codes_at + at + r * (HL / 2), *v = p + half_rec;
+			const uint32_t st = ring_at + stage * SL::kBytes;
+#pragma unroll
+			for (int q = 0; q < CH; q++) {
+				copy16(st + 512 * q, p + 512 * q);
+				copy16(st + SL::kVC + 512 * q, v + 512 * q);
+			}
+			if (lane < 2 * SLN)
+				copy16(to_scales + stage * SL::kBytes, scales_at + at + r * NB * 2);
+			ring_have |= 3u << 2 * stage;
+			return;
+		}
 		int pb = pa;
 		if (small)
 			pb = __shfl_sync(0xffffffffu, page_b, i & 31);
@@ -534,14 +564,18 @@ __global__ void __launch_bounds__(kAttnThreads, ATTN_MINB) kv_attn_kernel(AttnAr
 		bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
 		const float top = __uint_as_float(bits);
 		const bool bad = bits >= 0x7f800000u;
-		const int e = top > 0.0f && !bad ? 13 - ilogbf(top) : 0;   // -114 .. 162
-		const float up0 = __int_as_float((127 + e / 2) << 23);
-		const float up1 = __int_as_float((127 + e - e / 2) << 23);
+		const int e = top == 0.0f || bad ? 0 : 13 - ilogbf(top);   // -114 .. 162
+		const float up = __int_as_float((127 + min(e, 127)) << 23);
+		if (e > 127) {
+#pragma unroll
+			for (int k = 0; k < HL / 4; k++)
+				x[k] *= __int_as_float((e - 127 + 127) << 23);
+		}
 		// a query with an infinity or a NaN has no finite scores: NaN
 		const float qs = bad ? __int_as_float(0x7fffffff) : scalbnf(a.scale2 * kCodeUnit, -e);
 #pragma unroll
 		for (int k = 0; k < HL / 4; k++) {
-			const float v = bad ? 0.0f : x[k] * up0 * up1;
+			const float v = bad ? 0.0f : x[k] * up;
 			const float hi = __half2float(__float2half_rn(v));
 			x[k] = SPLIT && (g & 1) ? v - hi : hi;
 		}
@@ -552,7 +586,7 @@ __global__ void __launch_bounds__(kAttnThreads, ATTN_MINB) kv_attn_kernel(AttnAr
 				float t = 0.0f;
 #pragma unroll
 				for (int k = 0; k < 8; k++)
-					t += __half2float(__float2half_rn(x[8 * b + k]));
+					t += SPLIT ? __half2float(__float2half_rn(x[8 * b + k])) : x[8 * b + k];
 				t += __shfl_xor_sync(0xffffffffu, t, 1);
 				t += __shfl_xor_sync(0xffffffffu, t, 2);
 				t *= -8.0f / kCodeUnit;
@@ -964,93 +998,106 @@ __global__ void __launch_bounds__(kAttnThreads, ATTN_MINB) kv_attn_kernel(AttnAr
 	}
 }
 
-// The runs of a query row joined: grid (query tile, row of it), the warps
-// taking the runs in turn.  A few dependent loads long, so the sums of a warp's
-// first runs leave before the factors are known.
+// The runs of a tile's query rows joined, a CTA a tile: each row by as many of its
+// warps as the rows leave it, which take the runs in turn.  A few dependent loads
+// long, so the sums of a warp's first runs leave before the factors are known.
+constexpr int kMergeWarps = 16;
 template <typename T, int HL, int RPT>
-__global__ void __launch_bounds__(kAttnThreads) kv_merge_kernel(AttnArgs a)
+__global__ void __launch_bounds__(32 * kMergeWarps) kv_merge_kernel(AttnArgs a)
 {
 	constexpr int OS = HL + 4, E4 = HL / 4;                  // float4s of a row
 	constexpr int W = E4 < 32 ? E4 : 32, SIDE = 32 / W, NV = E4 / W;
 	constexpr int BATCH = 4;
-	__shared__ float4 red[kAttnWarps][E4];
+	__shared__ float4 red[kMergeWarps][E4];
 	Item it;
-	const bool mine = find_item<RPT, false>(a, blockIdx.x, it) && it.runs > 1;
+	const bool mine = cta_item<RPT, false>(a, blockIdx.x, it) && it.runs > 1;
 	griddep_wait();   // the runs are written
-	const int r = blockIdx.y;
-	if (!mine || r >= it.rows)
+	if (!mine)
 		return;
 	const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+	int share = kMergeWarps;   // warps of a row
+	while (share > 1 && share * it.rows > kMergeWarps)
+		share /= 2;
+	const int part = warp % share, ds = share * SIDE;
 	const int64_t step = (int64_t)a.KVH * a.part_rows * OS;   // between the runs of a tile
-	const float *pp = a.part + ((int64_t)it.first * a.part_rows + r) * OS;
-	const int s0 = warp * SIDE + lane / W, e = lane % W * 4;
-	constexpr int ds = kAttnWarps * SIDE;
-	float4 x[BATCH][NV];
-	float xb[BATCH];
-	auto load = [&](int s) {
+	for (int r0 = 0; r0 < it.rows; r0 += kMergeWarps / share) {
+		const int r = r0 + warp / share;
+		const bool row = r < it.rows;   // the whole warp
+		const float *pp = a.part + ((int64_t)it.first * a.part_rows + (row ? r : 0)) * OS;
+		const int s0 = part * SIDE + lane / W, e = lane % W * 4;
+		const int runs = row ? it.runs : 0;
+		float4 x[BATCH][NV], o[NV];
+		float xb[BATCH];
+		auto load = [&](int s) {
 #pragma unroll
-		for (int k = 0; k < BATCH; k++) {
-			const float *p = pp + (s + k * ds) * step;
-			const bool in = s + k * ds < it.runs;
-			xb[k] = in ? p[HL] : kNoMax;
+			for (int k = 0; k < BATCH; k++) {
+				const float *p = pp + (s + k * ds) * step;
+				const bool in = s + k * ds < runs;
+				xb[k] = in ? p[HL] : kNoMax;
 #pragma unroll
-			for (int v = 0; v < NV; v++)
-				x[k][v] = in ? *reinterpret_cast<const float4 *>(p + e + 4 * W * v)
-					     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+				for (int v = 0; v < NV; v++)
+					x[k][v] = in ? *reinterpret_cast<const float4 *>(p + e + 4 * W * v)
+						     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+			}
+		};
+		load(s0);
+		float b = kNoMax, l = 0.0f;
+		for (int s = lane; s < runs; s += 32)
+			b = fminf(b, pp[s * step + HL]);
+		b = -warp_max(-b);
+		for (int s = lane; s < runs; s += 32)
+			l += pp[s * step + HL + 1] * ex2(b - pp[s * step + HL]);
+		l = warp_sum(l);
+#pragma unroll
+		for (int v = 0; v < NV; v++)
+			o[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+		for (int s = s0;;) {
+#pragma unroll
+			for (int k = 0; k < BATCH; k++) {
+				const float f = ex2(b - xb[k]);
+#pragma unroll
+				for (int v = 0; v < NV; v++) {
+					o[v].x = fmaf(x[k][v].x, f, o[v].x);
+					o[v].y = fmaf(x[k][v].y, f, o[v].y);
+					o[v].z = fmaf(x[k][v].z, f, o[v].z);
+					o[v].w = fmaf(x[k][v].w, f, o[v].w);
+				}
+			}
+			s += BATCH * ds;
+			if (s - lane / W >= runs)
+				break;
+			load(s);
 		}
-	};
-	load(s0);
-	float b = kNoMax;
-	for (int s = lane; s < it.runs; s += 32)
-		b = fminf(b, pp[s * step + HL]);
-	b = -warp_max(-b);
-	float l = 0.0f;
-	for (int s = lane; s < it.runs; s += 32)
-		l += pp[s * step + HL + 1] * ex2(b - pp[s * step + HL]);
-	l = warp_sum(l);
-	float4 o[NV];
 #pragma unroll
-	for (int v = 0; v < NV; v++)
-		o[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-	for (int s = s0;; load(s)) {
+		for (int v = 0; v < NV; v++) {
+			if (SIDE == 2) {
+				o[v].x += __shfl_xor_sync(0xffffffffu, o[v].x, 16);
+				o[v].y += __shfl_xor_sync(0xffffffffu, o[v].y, 16);
+				o[v].z += __shfl_xor_sync(0xffffffffu, o[v].z, 16);
+				o[v].w += __shfl_xor_sync(0xffffffffu, o[v].w, 16);
+			}
+			if (share > 1 && lane < W)
+				red[warp][lane + W * v] = o[v];
+		}
+		if (share > 1) {   // one round of rows then: share * rows <= the warps
+			__syncthreads();
+			if (part == 0 && lane < W) {
 #pragma unroll
-		for (int k = 0; k < BATCH; k++) {
-			const float f = ex2(b - xb[k]);
-#pragma unroll
-			for (int v = 0; v < NV; v++) {
-				o[v].x = fmaf(x[k][v].x, f, o[v].x);
-				o[v].y = fmaf(x[k][v].y, f, o[v].y);
-				o[v].z = fmaf(x[k][v].z, f, o[v].z);
-				o[v].w = fmaf(x[k][v].w, f, o[v].w);
+				for (int v = 0; v < NV; v++)
+					for (int w = 1; w < share; w++) {
+						const float4 y = red[warp + w][lane + W * v];
+						o[v].x += y.x;
+						o[v].y += y.y;
+						o[v].z += y.z;
+						o[v].w += y.w;
+					}
 			}
 		}
-		s += BATCH * ds;
-		if (s - lane / W >= it.runs)
-			break;
-	}
+		if (row && part == 0 && lane < W) {
 #pragma unroll
-	for (int v = 0; v < NV; v++) {
-		if (SIDE == 2) {
-			o[v].x += __shfl_xor_sync(0xffffffffu, o[v].x, 16);
-			o[v].y += __shfl_xor_sync(0xffffffffu, o[v].y, 16);
-			o[v].z += __shfl_xor_sync(0xffffffffu, o[v].z, 16);
-			o[v].w += __shfl_xor_sync(0xffffffffu, o[v].w, 16);
+			for (int v = 0; v < NV; v++)
+				write_row<T>(a, it, r, e + 4 * W * v, o[v], b, l, e + 4 * W * v == 0);
 		}
-		if (lane < W)
-			red[warp][lane + W * v] = o[v];
-	}
-	__syncthreads();
-	if (threadIdx.x < E4) {
-		float4 v = red[0][threadIdx.x];
-#pragma unroll
-		for (int w = 1; w < kAttnWarps; w++) {
-			const float4 y = red[w][threadIdx.x];
-			v.x += y.x;
-			v.y += y.y;
-			v.z += y.z;
-			v.w += y.w;
-		}
-		write_row<T>(a, it, r, 4 * threadIdx.x, v, b, l, threadIdx.x == 0);
 	}
 }
 
@@ -1113,8 +1160,8 @@ cudaError_t launch_attn_as(const AttnArgs &a, const Plan &p, cudaStream_t st)
 	if (!p.split)
 		return cudaSuccess;
 	cudaLaunchConfig_t cfg{};
-	cfg.gridDim = dim3((unsigned)p.tiles, p.rows < RPT ? p.rows : RPT);
-	cfg.blockDim = dim3(kAttnThreads);
+	cfg.gridDim = dim3((unsigned)p.tiles);
+	cfg.blockDim = dim3(32 * kMergeWarps);
 	cfg.stream = st;
 	cudaLaunchAttribute at[1];
 	at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
