@@ -41,11 +41,27 @@ namespace {
 constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps;
 constexpr int kAttnTile = 32;      // key rows of a warp's copy
 constexpr int kAttnStages = 3;     // copies in a warp's ring
-constexpr int kRunMin = kAttnWarps;          // tiles of a run: one for each warp
-constexpr int kRunMax = 256 * kAttnWarps;    // 512 products a warp in one fp32 chain
+constexpr int kRunMin = 1;         // tiles of a run
+constexpr int kRunMax = 256;       // 512 products in one fp32 chain
 constexpr float kLag = 4.0f;       // exponents of 2 that the running maximum may lag
 constexpr float kLift = 10.0f;     // weights are held times 2^10
 constexpr float kNoMax = 3.0e38f;  // the bias kLift - m before any row was seen
+
+// j / n and j % n for any 31-bit j: the quotient by a rounded-down reciprocal is at
+// most one short.  (A division by a runtime value is some twenty dependent
+// instructions, which a decode step's few warps wait for.)
+struct QuickDiv {
+	unsigned n = 1, m = 0;
+	QuickDiv() {}
+	explicit QuickDiv(unsigned n_) : n(n_), m(n_ > 1 ? (unsigned)(0x100000000ull / n_) : 0) {}
+	__device__ __forceinline__ int div(int j) const
+	{
+		if (n == 1)
+			return j;
+		const unsigned q = __umulhi((unsigned)j, m);
+		return (int)(q + ((unsigned)j - q * n >= n));
+	}
+};
 
 struct AttnArgs {
 	BatchArgs b;
@@ -56,6 +72,7 @@ struct AttnArgs {
 	const uint8_t *pages;
 	int64_t page_bytes;
 	int H, KVH, G;
+	QuickDiv by_g, by_kvh;
 	int causal, window;
 	float scale2;        // scale * log2 e
 	int q_vec, o_vec;    // 16-byte aligned rows
@@ -86,7 +103,7 @@ __device__ __forceinline__ bool seq_of(const AttnArgs &a, int b, int &s0, int &n
 			kv <= a.b.max_kv && (b > 0 || s0 == 0);
 	if (!ok) {
 		n = 0;
-		if (blockIdx.x == 0)
+		if (blockIdx.x == 0 && threadIdx.x < 32)
 			atomicOr(a.b.err, kKvErrBatch);
 	}
 	return ok;
@@ -164,7 +181,7 @@ __device__ __forceinline__ bool find_item(const AttnArgs &a, int index, Item &f)
 			f.s0 = s0;
 			f.n = n;
 			f.kv = kv;
-			const unsigned rest = at / (unsigned)a.KVH;
+			const unsigned rest = a.by_kvh.div(at);
 			f.kvh = at - rest * a.KVH;
 			const unsigned rank = ITEM ? rest / (unsigned)runs : rest;
 			f.run = ITEM ? rest - rank * (unsigned)runs : 0;
@@ -172,7 +189,7 @@ __device__ __forceinline__ bool find_item(const AttnArgs &a, int index, Item &f)
 			f.tile = tiles - 1 - (int)rank;
 			f.r0 = f.tile * RPT;
 			f.rows = min(RPT, n * a.G - f.r0);
-			const int p0 = kv - n + f.r0 / a.G, p1 = kv - n + (f.r0 + f.rows - 1) / a.G;
+			const int p0 = kv - n + a.by_g.div(f.r0), p1 = kv - n + a.by_g.div(f.r0 + f.rows - 1);
 			f.lo = a.window ? max(0, p0 - a.window + 1) : 0;
 			f.hi = a.causal ? min(kv, p1 + 1) : kv;
 			const int ta = f.lo / kAttnTile, tb = max(ta, (f.hi + kAttnTile - 1) / kAttnTile);
@@ -327,35 +344,43 @@ __device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[NW])
 	}
 }
 
-// values e .. e + 3 of row r of a tile: the sums over the weights' sum, and
-// with e 0 the row's log-sum-exp
+// Row r of a tile as it leaves: sums over the weights' sum, zeros where nothing was
+// seen, and its log-sum-exp
 template <typename T>
-__device__ __forceinline__ void write_row(const AttnArgs &a, const Item &it, int r, int e, float4 v,
-					  float b, float l, bool first)
-{
-	const int qr = it.r0 + r, token = it.s0 + qr / a.G, head = it.kvh * a.G + qr % a.G;
-	// nothing seen: zeros
-	const float il = l == 0.0f ? 0.0f : 1.0f / l;
-	T *p = static_cast<T *>(a.out) + token * a.o_ts + head * a.o_hs + e;
-	const float x[4] = {v.x * il, v.y * il, v.z * il, v.w * il};
-	if (a.o_vec && sizeof(T) == 4) {
-		*reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
-	} else if (a.o_vec) {
-		uint2 u;
-		T *h = reinterpret_cast<T *>(&u);
-#pragma unroll
-		for (int k = 0; k < 4; k++)
-			h[k] = from_f32<T>(x[k]);
-		*reinterpret_cast<uint2 *>(p) = u;
-	} else {
-#pragma unroll
-		for (int k = 0; k < 4; k++)
-			p[k] = from_f32<T>(x[k]);
+struct RowOut {
+	T *p;
+	float *lse_at;
+	float il, l, bias;
+	bool vec;
+	__device__ __forceinline__ RowOut(const AttnArgs &a, const Item &it, int r, float bias_, float l_)
+		: il(l_ == 0.0f ? 0.0f : 1.0f / l_), l(l_), bias(bias_), vec(a.o_vec)
+	{
+		const int qr = it.r0 + r, i = a.by_g.div(qr);
+		const int token = it.s0 + i, head = it.kvh * a.G + qr - i * a.G;
+		p = static_cast<T *>(a.out) + token * a.o_ts + head * a.o_hs;
+		lse_at = a.lse ? a.lse + (int64_t)token * a.H + head : nullptr;
 	}
-	if (first && a.lse)
-		a.lse[(int64_t)token * a.H + head] =
-			l == 0.0f ? -__int_as_float(0x7f800000) : 0.693147180559945f * (log2f(l) - b);
-}
+	__device__ __forceinline__ void two(int e, float x, float y) const
+	{
+		x *= il;
+		y *= il;
+		if (!vec) {
+			p[e] = from_f32<T>(x);
+			p[e + 1] = from_f32<T>(y);
+		} else if constexpr (sizeof(T) == 4) {
+			*reinterpret_cast<float2 *>(p + e) = make_float2(x, y);
+		} else {
+			T v[2] = {from_f32<T>(x), from_f32<T>(y)};
+			*reinterpret_cast<uint32_t *>(p + e) = *reinterpret_cast<uint32_t *>(v);
+		}
+	}
+	__device__ __forceinline__ void lse() const
+	{
+		if (lse_at)
+			*lse_at = l == 0.0f ? -__int_as_float(0x7f800000)
+					    : 0.693147180559945f * (log2f(l) - bias);
+	}
+};
 
 template <int HL>
 struct StageLayout {
@@ -365,13 +390,8 @@ struct StageLayout {
 	static constexpr int kBytes = 2 * (kCodes + kScales);
 };
 
-template <int HL, int NT>
-constexpr int attn_smem()
-{
-	constexpr int ring = kAttnWarps * kAttnStages * StageLayout<HL>::kBytes;
-	constexpr int join = kAttnWarps * 8 * NT * (HL + 4) * 4;
-	return ring > join ? ring : join;
-}
+template <int HL>
+constexpr int kAttnSmem = kAttnWarps * kAttnStages * StageLayout<HL>::kBytes;
 
 #ifndef ATTN_MINB
 #define ATTN_MINB (HL == 128 && NT == 1 ? 4 : 1)
@@ -397,30 +417,29 @@ __global__ void __launch_bounds__(kAttnThreads, ATTN_MINB) kv_attn_kernel(AttnAr
 {
 	constexpr bool SPLIT = sizeof(T) == 4;        // two columns a row
 	constexpr int RPN = SPLIT ? 4 : 8;            // rows of an 8-column tile
-	constexpr int RPT = RPN * NT, NB = HL / 32, COLS = 8 * NT;
+	constexpr int RPT = RPN * NT, NB = HL / 32;
 	constexpr bool QR = kQInRegs<HL, NT>;
 	// one column tile: the keys' -8 sum to -8 sum q, where the scores' sums start
 	constexpr bool KRAW = NT == 1;
 	using SL = StageLayout<HL>;
 	extern __shared__ __align__(128) uint8_t smem[];
-	__shared__ float sm_b[kAttnWarps][COLS], sm_l[kAttnWarps][COLS];
-	__shared__ uint2 sm_q[QR ? 1 : 2 * NB * NT][32];
-	__shared__ float sm_qs[COLS];
+	__shared__ uint2 sm_q[kAttnWarps][QR ? 1 : 2 * NB * NT][32];
 	const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
 
 	griddep_launch_dependents();
 	Item it;
-	if (!cta_item<RPT, true>(a, blockIdx.x, it))
+	const int item = blockIdx.x * kAttnWarps + warp;
+	if (!find_item<RPT, true>(a, item, it))
 		return;
 
-	// ---- the warp's key tiles: t0 + warp, + 4, ..: lane l keeps the pages of
-	// the next 32 of them (two where a page is half a tile)
-	const int ntile = max(0, (it.t1 - it.t0 - warp + kAttnWarps - 1) / kAttnWarps);
+	// ---- the key tiles t0, t0 + 1, ..: lane l keeps the pages of the next 32 of
+	// them (two where a page is half a tile)
+	const int ntile = it.t1 - it.t0;
 	const int32_t *table = a.b.table + it.b * a.b.table_stride;
 	const int P = 1 << a.b.page_log2;
 	const bool small = P < kAttnTile;
 	uint8_t *ring = smem + warp * kAttnStages * SL::kBytes;
-	auto key0 = [&](int i) { return (it.t0 + warp + i * kAttnWarps) * kAttnTile; };
+	auto key0 = [&](int i) { return (it.t0 + i) * kAttnTile; };
 	// which halves of tile i hold rows that the query tile sees
 	auto needs = [&](int k0) -> int {
 		return (k0 < it.hi && k0 + 16 > it.lo ? 1 : 0) |
@@ -520,16 +539,16 @@ __global__ void __launch_bounds__(kAttnThreads, ATTN_MINB) kv_attn_kernel(AttnAr
 	uint2 qf[QR ? 2 * NB * NT : 1];
 	float2 q_off[KRAW ? NB : 1];
 	const T *qp = static_cast<const T *>(a.q) + (int64_t)it.kvh * a.G * a.q_hs;
-	float qs_own[QR ? NT : 1];
+	// factors of the lane's columns 2 c, 2 c + 1 of each tile
+	float qs0[NT], qs1[NT];
 #pragma unroll
 	for (int nt = 0; nt < NT; nt++) {
-		if (!QR && nt % kAttnWarps != warp)
-			continue;   // one warp each, through shared memory
 		const int r = nt * RPN + (SPLIT ? g / 2 : g);
 		float x[HL / 4];
 		if (r < it.rows) {
 			const int qr = it.r0 + r;
-			const T *p = qp + (it.s0 + qr / a.G) * a.q_ts + (qr % a.G) * a.q_hs;
+			const int i = a.by_g.div(qr);
+			const T *p = qp + (it.s0 + i) * a.q_ts + (qr - i * a.G) * a.q_hs;
 #pragma unroll
 			for (int h = 0; h < HL / 16; h++) {
 				if (a.q_vec && sizeof(T) == 4) {
@@ -602,29 +621,13 @@ __global__ void __launch_bounds__(kAttnThreads, ATTN_MINB) kv_attn_kernel(AttnAr
 			if constexpr (QR)
 				qf[nt * 2 * NB + h] = f;
 			else
-				sm_q[nt * 2 * NB + h][lane] = f;
+				sm_q[warp][nt * 2 * NB + h][lane] = f;   // the lane's own
 		}
-		if constexpr (QR)
-			qs_own[nt] = qs;
-		else if (c == 0)
-			sm_qs[nt * 8 + g] = qs;
-	}
-	if constexpr (!QR)
-		__syncthreads();
-	// factors of this lane's columns 2 c, 2 c + 1 of each tile
-	float qs0[NT], qs1[NT];
-#pragma unroll
-	for (int nt = 0; nt < NT; nt++) {
-		if constexpr (QR) {
-			qs0[nt] = __shfl_sync(0xffffffffu, qs_own[nt], 8 * c);
-			qs1[nt] = __shfl_sync(0xffffffffu, qs_own[nt], 8 * c + 4);
-		} else {
-			qs0[nt] = sm_qs[nt * 8 + 2 * c];
-			qs1[nt] = sm_qs[nt * 8 + 2 * c + 1];
-		}
+		qs0[nt] = __shfl_sync(0xffffffffu, qs, 8 * c);
+		qs1[nt] = __shfl_sync(0xffffffffu, qs, 8 * c + 4);
 	}
 	// the cache row at which each column's query stands
-	auto row_of = [&](int r) { return it.kv - it.n + (it.r0 + r) / a.G; };
+	auto row_of = [&](int r) { return it.kv - it.n + a.by_g.div(it.r0 + r); };
 	auto row0 = [&](int nt) { return row_of(nt * RPN + (SPLIT ? c : 2 * c)); };
 	auto row1 = [&](int nt) { return row_of(nt * RPN + (SPLIT ? c : 2 * c + 1)); };
 	const int first_row = row_of(0), last_row = row_of(it.rows - 1);
@@ -705,8 +708,8 @@ __global__ void __launch_bounds__(kAttnThreads, ATTN_MINB) kv_attn_kernel(AttnAr
 						q0 = qf[nt * 2 * NB + 2 * b];
 						q1 = qf[nt * 2 * NB + 2 * b + 1];
 					} else {
-						q0 = sm_q[nt * 2 * NB + 2 * b][lane];
-						q1 = sm_q[nt * 2 * NB + 2 * b + 1][lane];
+						q0 = sm_q[warp][nt * 2 * NB + 2 * b][lane];
+						q1 = sm_q[warp][nt * 2 * NB + 2 * b + 1][lane];
 					}
 					float d[4];
 					if constexpr (KRAW)
@@ -925,83 +928,55 @@ __global__ void __launch_bounds__(kAttnThreads, ATTN_MINB) kv_attn_kernel(AttnAr
 	}
 	copies_wait<0>();
 
-	// ---- the warps' sums joined, over the ring's memory
+	// ---- out of the registers: a lane has values 2 g, 2 g + 1 of every half block
+	// of its columns' rows, 8 lanes 16 values side by side
+	constexpr int OS = HL + 4;
+	float iv[NB];   // sums in true size: the codes' unit, the V scales' factors
+#pragma unroll
+	for (int b = 0; b < NB; b++)
+		iv[b] = kCodeUnit / half_of(v_fac[b / 2], b & 1);
 #pragma unroll
 	for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
 		for (int x = 4; x < 32; x *= 2) {
 			l0[nt] += __shfl_xor_sync(0xffffffffu, l0[nt], x);
-			l1[nt] += __shfl_xor_sync(0xffffffffu, l1[nt], x);
+			if (!SPLIT)
+				l1[nt] += __shfl_xor_sync(0xffffffffu, l1[nt], x);
 		}
-		if (SPLIT)
-			l1[nt] = l0[nt];
-		if (g == 0) {
-			sm_b[warp][nt * 8 + 2 * c] = b0[nt];
-			sm_b[warp][nt * 8 + 2 * c + 1] = b1[nt];
-			sm_l[warp][nt * 8 + 2 * c] = l0[nt];
-			sm_l[warp][nt * 8 + 2 * c + 1] = l1[nt];
-		}
-	}
-	__syncthreads();
-	auto bias_of = [&](int col) {   // of the largest maximum
-		float b = sm_b[0][col];
 #pragma unroll
-		for (int w = 1; w < kAttnWarps; w++)
-			b = fminf(b, sm_b[w][col]);
-		return b;
-	};
-	constexpr int OS = HL + 4;
-	float *ob = reinterpret_cast<float *>(smem);
+		for (int h = 0; h < (SPLIT ? 1 : 2); h++) {   // the columns' rows: one, or two
+			const int r = nt * RPN + (SPLIT ? c : 2 * c + h);
+			if (r >= it.rows)
+				continue;
+			const float l = h ? l1[nt] : l0[nt], bias = h ? b1[nt] : b0[nt];
+			auto value = [&](int k, int i) {   // i: the first or second of the two
+				const float v = SPLIT ? o[k][nt][2 * i] + o[k][nt][2 * i + 1] : o[k][nt][2 * i + h];
+				return v * (k & 1 ? iv[k / 2] * 0.0625f : iv[k / 2]);
+			};
+			if (it.runs > 1) {
+				float *pp = a.part + ((int64_t)item * a.part_rows + r) * OS;
 #pragma unroll
-	for (int nt = 0; nt < NT; nt++) {
-		const int col = nt * 8 + 2 * c;
-		const float f0 = ex2(bias_of(col) - b0[nt]), f1 = ex2(bias_of(col + 1) - b1[nt]);
-		float *o0 = ob + (warp * COLS + col) * OS, *o1 = o0 + OS;
+				for (int k = 0; k < 2 * NB; k++)
+					*reinterpret_cast<float2 *>(pp + 16 * k + 2 * g) =
+						make_float2(value(k, 0), value(k, 1));
+				if (g == 0)
+					*reinterpret_cast<float2 *>(pp + HL) = make_float2(bias, l);
+			} else {
+				const RowOut<T> out(a, it, r, bias, l);
 #pragma unroll
-		for (int k = 0; k < 2 * NB; k++) {
-			const float iv = (k & 1 ? kCodeUnit / 16 : kCodeUnit) / half_of(v_fac[k / 4], k / 2 & 1);
-			const int e = 32 * (k / 2) + 16 * (k & 1) + 2 * g;
-			*reinterpret_cast<float2 *>(o0 + e) =
-				make_float2(o[k][nt][0] * f0 * iv, o[k][nt][2] * f0 * iv);
-			*reinterpret_cast<float2 *>(o1 + e) =
-				make_float2(o[k][nt][1] * f1 * iv, o[k][nt][3] * f1 * iv);
-		}
-	}
-	__syncthreads();
-	for (int i = threadIdx.x; i < it.rows * (HL / 4); i += kAttnThreads) {
-		const int r = i / (HL / 4), e = i % (HL / 4) * 4;
-		const int col = SPLIT ? r / RPN * 8 + 2 * (r % RPN) : r;
-		const float b = bias_of(col);
-		float l = 0.0f;
-		float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-		for (int w = 0; w < kAttnWarps; w++) {
-			l += sm_l[w][col] * ex2(b - sm_b[w][col]);
-#pragma unroll
-			for (int h = 0; h < (SPLIT ? 2 : 1); h++) {
-				const float4 x =
-					*reinterpret_cast<const float4 *>(ob + (w * COLS + col + h) * OS + e);
-				v.x += x.x;
-				v.y += x.y;
-				v.z += x.z;
-				v.w += x.w;
+				for (int k = 0; k < 2 * NB; k++)
+					out.two(16 * k + 2 * g, value(k, 0), value(k, 1));
+				if (g == 0)
+					out.lse();
 			}
-		}
-		if (it.runs > 1) {
-			float *pp = a.part + ((int64_t)blockIdx.x * a.part_rows + r) * OS;
-			*reinterpret_cast<float4 *>(pp + e) = v;
-			if (e == 0)
-				*reinterpret_cast<float2 *>(pp + HL) = make_float2(b, l);
-		} else {
-			write_row<T>(a, it, r, e, v, b, l, e == 0);
 		}
 	}
 }
 
-// The runs of a tile's query rows joined, a CTA a tile: each row by as many of its
-// warps as the rows leave it, which take the runs in turn.  A few dependent loads
+// The runs of a tile's query rows joined, a CTA a tile or some rows of it: each
+// row by as many of its warps as the rows leave it, which take the runs in turn.  A few dependent loads
 // long, so the sums of a warp's first runs leave before the factors are known.
-constexpr int kMergeWarps = 16;
+constexpr int kMergeWarps = 4;
 template <typename T, int HL, int RPT>
 __global__ void __launch_bounds__(32 * kMergeWarps) kv_merge_kernel(AttnArgs a)
 {
@@ -1015,14 +990,17 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv_merge_kernel(AttnArgs a)
 	if (!mine)
 		return;
 	const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-	int share = kMergeWarps;   // warps of a row
-	while (share > 1 && share * it.rows > kMergeWarps)
+	// the CTA's rows of the tile; warps of a row
+	const int each = (a.part_rows + gridDim.y - 1) / gridDim.y;
+	const int from = blockIdx.y * each, to = min(from + each, it.rows);
+	int share = kMergeWarps;
+	while (share > 1 && share * (to - from) > kMergeWarps)
 		share /= 2;
 	const int part = warp % share, ds = share * SIDE;
 	const int64_t step = (int64_t)a.KVH * a.part_rows * OS;   // between the runs of a tile
-	for (int r0 = 0; r0 < it.rows; r0 += kMergeWarps / share) {
+	for (int r0 = from; r0 < to; r0 += kMergeWarps / share) {
 		const int r = r0 + warp / share;
-		const bool row = r < it.rows;   // the whole warp
+		const bool row = r < to;   // the whole warp
 		const float *pp = a.part + ((int64_t)it.first * a.part_rows + (row ? r : 0)) * OS;
 		const int s0 = part * SIDE + lane / W, e = lane % W * 4;
 		const int runs = row ? it.runs : 0;
@@ -1094,9 +1072,14 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv_merge_kernel(AttnArgs a)
 			}
 		}
 		if (row && part == 0 && lane < W) {
+			const RowOut<T> out(a, it, r, b, l);
 #pragma unroll
-			for (int v = 0; v < NV; v++)
-				write_row<T>(a, it, r, e + 4 * W * v, o[v], b, l, e + 4 * W * v == 0);
+			for (int v = 0; v < NV; v++) {
+				out.two(e + 4 * W * v, o[v].x, o[v].y);
+				out.two(e + 4 * W * v + 2, o[v].z, o[v].w);
+			}
+			if (lane == 0)
+				out.lse();
 		}
 	}
 }
@@ -1126,9 +1109,9 @@ Plan plan_of(const moe_kv_cache *c, const moe_kv_batch *b, int64_t H, bool fp32)
 	const int64_t by_token = b->n_tokens * G / p.rpt + b->n_seqs;
 	p.tiles = KVH * (by_seq < by_token ? by_seq : by_token);
 	p.rows = (int)(rows < p.rpt ? rows : p.rpt);
-	// items for whole waves of resident CTAs (4 an SM, fewer for wide tiles), the
+	// items for whole waves of resident warps (16 an SM, fewer for wide tiles), the
 	// runs' remainders among them (a remainder a query tile at most)
-	const int64_t wave = (int64_t)sm_count() * (HL * p.nt <= 128 ? 4 : 2);
+	const int64_t wave = (int64_t)sm_count() * kAttnWarps * (HL * p.nt <= 128 ? 4 : 2);
 	int64_t want = wave - p.tiles;
 	while (want < wave / 2)
 		want += wave;
@@ -1151,16 +1134,19 @@ template <typename T, int HL, int NT>
 cudaError_t launch_attn_as(const AttnArgs &a, const Plan &p, cudaStream_t st)
 {
 	constexpr int RPT = (sizeof(T) == 4 ? 4 : 8) * NT;
-	constexpr int smem = attn_smem<HL, NT>();
+	constexpr int smem = kAttnSmem<HL>;
 	if (cudaError_t e = ensure_smem(kv_attn_kernel<T, HL, NT>, smem))
 		return e;
-	kv_attn_kernel<T, HL, NT><<<(unsigned)p.items, kAttnThreads, smem, st>>>(a);
+	kv_attn_kernel<T, HL, NT>
+		<<<(unsigned)((p.items + kAttnWarps - 1) / kAttnWarps), kAttnThreads, smem, st>>>(a);
 	if (cudaError_t e = cudaGetLastError())
 		return e;
 	if (!p.split)
 		return cudaSuccess;
 	cudaLaunchConfig_t cfg{};
-	cfg.gridDim = dim3((unsigned)p.tiles);
+	// few tiles: their rows over several CTAs, up to one a row
+	const int64_t y = 8 * (int64_t)sm_count() / p.tiles;
+	cfg.gridDim = dim3((unsigned)p.tiles, (unsigned)(y < 1 ? 1 : y < p.rows ? y : p.rows));
 	cfg.blockDim = dim3(32 * kMergeWarps);
 	cfg.stream = st;
 	cudaLaunchAttribute at[1];
@@ -1277,6 +1263,8 @@ int moe_kv_attention(moe_kv_cache *cache, const moe_kv_batch *batch, const moe_r
 	a.H = (int)q->n_heads;
 	a.KVH = (int)KVH;
 	a.G = (int)(q->n_heads / KVH);
+	a.by_g = QuickDiv((unsigned)a.G);
+	a.by_kvh = QuickDiv((unsigned)KVH);
 	a.causal = causal != 0;
 	a.window = (int)window;
 	a.scale2 = scale * 1.44269504088896f;
