@@ -409,7 +409,8 @@ typedef struct moe_rope_desc {
  * bytes. */
 MOE_API int moe_rope_create(moe_rope **out, const moe_rope_desc *desc);
 MOE_API int moe_rope_destroy(moe_rope *rope);
-/* q_out = q turned by pos[t] and, where k is not NULL, k_out = k turned: the
+/* (n_tokens <= 2^30, head_len <= 4096, and heads * head_len <= 2^19 as for every
+ * moe_rows) q_out = q turned by pos[t] and, where k is not NULL, k_out = k turned: the
  * first rot of every head's head_len values turn, the rest are copied.  fp32
  * arithmetic (each product and sum rounded once), rounded once to the rows'
  * type, which is one for all four.  An output may be its own input (same data
@@ -426,8 +427,9 @@ MOE_API int moe_rope_status(moe_rope *rope);
  * and values of n_kv_heads heads in 4 bits.  A row of head_len values is cut
  * into nb = head_len / 32 blocks of 32: value = scale * (code - 8), with
  *   scale = fp16(-m / 8), m the block's largest value or, where its magnitude is
- *           larger, its smallest, held to +-65504 (+0 for either zero); NaN where a value of the block
- *           is not finite (a poisoned block reads as NaN, not as a number),
+ *           larger, its smallest, held to +-65504 (+0 for either zero); NaN where a
+ *           value of the block is not finite (a poisoned block reads as NaN, not as
+ *           a number),
  *   code  = rint(value * (1 / scale)) + 8 held to 0 .. 15 (8 where scale is 0).
  * Byte k of a block has the code of value k in its low nibble and of value k + 16
  * in its high nibble, as in Q4_0.  In memory, per page and KV head:
@@ -491,12 +493,15 @@ MOE_API int moe_kv_gather(moe_kv_cache *cache, const moe_kv_batch *batch, const 
  * at cache row p sees rows j <= p, and with window > 0 only j > p - window
  * (causal only; 0: all).  A query that sees no row gives zeros.  lse (fp32
  * [n_tokens, n_heads], or NULL) receives ln sum_j exp(score), -infinity where
- * nothing is seen.  q and out have one type.  Products take the codes exactly, q
- * and the weights in fp16 (fp32 rows: as two fp16 halves, about 22 bits); sums
- * and softmax statistics are fp32.  Rows that a query does not see never reach
+ * nothing is seen.  q and out have one type; out may be q itself (same data and
+ * strides) and must not overlap it otherwise.  Products take the codes exactly, q
+ * in fp16 after a power of two a row, and the weights in fp16, rounded once and
+ * once more with V's scale (fp32 rows: q and weights as two fp16 halves, about 22
+ * bits); sums and softmax statistics are fp32.  Rows that a query does not see never reach
  * its result, whatever they hold.
  * workspace: 16-byte aligned, at least moe_kv_attention_workspace bytes (which
- * follow from the batch's four sizes); used by this call only. */
+ * follow from n_heads, the cache and the batch's n_seqs, n_tokens, max_q and
+ * max_kv; 0: none needed); what it holds counts for this call only. */
 MOE_API int64_t moe_kv_attention_workspace(const moe_kv_cache *cache, const moe_kv_batch *batch,
 					   int64_t n_heads);
 MOE_API int moe_kv_attention(moe_kv_cache *cache, const moe_kv_batch *batch, const moe_rows *q,

@@ -526,10 +526,12 @@ struct PairItem {
 };
 
 // How a packed batch is cut into CTAs of 8 warps (a token's items are `rounds` warps
-// of them): as many tokens to a CTA (up to kGroupTokens, and 2048 angles) as leave one
-// wave of resident CTAs, so that the look-ups and angles that a CTA waits for are
-// paid once for much work; few tokens: several warps and CTAs a token.  Powers of
-// two, for the divisions that a decode step would wait for.
+// of them): as many tokens to a CTA (up to kGroupTokens, and 2048 angles) as leave a
+// wave and a half of resident CTAs, so that the look-ups and angles that a CTA waits
+// for are paid once for much work.  Against 1 and 2 waves: 2048 tokens' rotation 17.2
+// us (17.3, 18.5), 16383 tokens' 58.8 (59.8, 59.1), 16383 appended 54.2 (57.6, 54.0).
+// Few tokens: several warps and CTAs a token.  Powers of two, for the divisions that
+// a decode step would wait for.
 constexpr int kGroupTokens = 32;
 struct TokenSplit {
 	int tokens;       // of a CTA: 1, 2, 4 or a multiple of 8
@@ -539,7 +541,7 @@ struct TokenSplit {
 inline TokenSplit split_tokens(int64_t n_tokens, int64_t rounds, int half)
 {
 	const int64_t wave = 4 * (int64_t)sm_count();
-	int64_t tokens = (n_tokens + wave - 1) / wave;
+	int64_t tokens = (2 * n_tokens + 3 * wave - 1) / (3 * wave);
 	tokens = tokens < kGroupTokens ? tokens : kGroupTokens;
 	while (tokens > 1 && tokens * half > 2048)
 		tokens--;
@@ -563,14 +565,15 @@ __device__ __forceinline__ Rounds::Rounds(const TokenSplit &s, int slice)
 }
 
 // A warp's rows in flight to slots of its own in shared memory, kDepth rounds of them:
-// loads that hold no registers, so that a warp keeps 3 KB on the way whatever its
-// work needs (96 KB an SM).  Rounds come out in the order in which they went in.  A
-// lane gets 8 values side by side; those of fp32 rows are 32 bytes, which reach
-// memory as two times 16 that neighbouring lanes hold together (each 32-byte sector
-// once).  Rows that are not 16-byte aligned are read where they come out.
+// loads that hold no registers, so that a warp keeps 2 KB on the way whatever its work
+// needs (64 KB an SM; with 3 KB 16383 tokens take 60.9 us instead of 59.8 to rotate).
+// Rounds come out in the order in which they went in.  A lane gets 8 values side by
+// side; those of fp32 rows are 32 bytes, which reach memory as two times 16 that
+// neighbouring lanes hold together (each 32-byte sector once).  Rows that are not
+// 16-byte aligned are read where they come out.
 template <typename T, bool VEC>
 struct RowStream {
-	static constexpr int kParts = 8 * sizeof(T) / 16, kDepth = 12 / (int)sizeof(T);
+	static constexpr int kParts = 8 * sizeof(T) / 16, kDepth = 8 / (int)sizeof(T);
 	static constexpr int kWarpBytes = VEC ? kDepth * kParts * 512 : 0;
 	uint32_t mine, part;   // the lane's 8 values of a slot, its 16 bytes of a row's first part
 	int across, jump;      // bytes from part to part, and from the values to part 0 in memory
@@ -708,6 +711,8 @@ struct RowReader {
 	}
 	__device__ __forceinline__ void begin()
 	{
+		if (w.left == 0)   // what another reader has begun stays next
+			return;
 #pragma unroll
 		for (int i = 0; i < RowStream<T, VEC>::kDepth; i++)
 			next();

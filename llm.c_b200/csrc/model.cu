@@ -1218,6 +1218,7 @@ int ensure_kv_ws(moe_model *m, int64_t T)
 		return MOE_OK;
 	MCK(cudaStreamSynchronize(m->st));
 	dfree(m, m->kv_ws, m->kv_ws_bytes);
+	m->kv_ws = nullptr;
 	m->kv_ws_bytes = 0;
 	MRC(dalloc(m, &m->kv_ws, (size_t)need));
 	m->kv_ws_bytes = (size_t)need;

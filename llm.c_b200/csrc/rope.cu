@@ -349,7 +349,7 @@ int moe_rope_forward(moe_rope *rope, int64_t n_tokens, int64_t head_len, const i
 	const char *what = "moe_rope_forward";
 	if (!rope)
 		return kv_fail(MOE_ERR_INVALID, "%s: null rope", what);
-	if (n_tokens < 0 || n_tokens > 0x7fffffff || head_len < rope->rot || head_len > 4096 ||
+	if (n_tokens < 0 || n_tokens > (1 << 30) || head_len < rope->rot || head_len > 4096 ||
 	    head_len % 2)
 		return kv_fail(MOE_ERR_INVALID, "%s: %lld tokens, head_len %lld (even, at least rot %lld, "
 			       "up to 4096)", what, (long long)n_tokens, (long long)head_len,
@@ -405,6 +405,7 @@ int moe_rope_status(moe_rope *rope)
 	if (!e)
 		return MOE_OK;
 	KV_CK(what, cudaMemset(rope->err, 0, 4));
+	KV_CK(what, cudaDeviceSynchronize());   // before a call on any stream records the next
 	return kv_fail(MOE_ERR_INVALID, "%s: a position was out of range", what);
 }
 

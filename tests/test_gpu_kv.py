@@ -101,6 +101,32 @@ def test_rope_scaling_far_positions(m, kw):
     assert torch.equal(out[:1], x[:1] * 0.5)   # position 0, magnitude a power of two
 
 
+@pytest.mark.parametrize("layout", ["pairs", "halves"])
+@pytest.mark.parametrize("T,H,KVH,D,rot", [(2500, 3, 1, 64, 64), (6001, 1, 1, 128, 64), (20000, 1, 0, 64, 32),
+                                            (2500, 1, 1, 256, 250), (9000, 2, 0, 66, 66)])
+def test_rope_many_tokens(m, T, H, KVH, D, rot, layout):
+    """tokens enough that a CTA takes 2, 4, 8 .. of them; rows at odd offsets and in place
+    have the aligned rows' bits"""
+    x = rand(T, T, H + KVH, D, dtype=torch.bfloat16).cuda()
+    pos = np.random.default_rng(T).integers(0, 4096, T)
+    p = cuda_i32(pos)
+    r = m.Rope(rot, 1e4, 4096, m.ROPE_PAIRS if layout == "pairs" else m.ROPE_HALVES)
+
+    def turn(a, b):
+        k = (rows(m, a[:, H:]), rows(m, b[:, H:])) if KVH else (None, None)
+        r.forward(T, D, p.data_ptr(), rows(m, a[:, :H]), rows(m, b[:, :H]), *k, stream=LEGACY)
+        assert r.status() == 0
+
+    out = torch.full_like(x, 5.0)
+    turn(x, out)
+    check_turned(out, x, pos, ref.frequencies(rot, 1e4), layout)
+    wide = torch.full((T, (H + KVH) * D + 3), 5.0, dtype=x.dtype, device="cuda")
+    odd = wide[:, 1:-2].unflatten(1, (H + KVH, D))
+    odd.copy_(x)
+    turn(odd, odd)
+    assert torch.equal(odd, out) and (wide[:, 0] == 5.0).all() and (wide[:, -2:] == 5.0).all()
+
+
 def test_rope_positions_out_of_range(m):
     """such a token stays unwritten and is reported once; the others turn"""
     r = m.Rope(64, 1e4, 100)
@@ -285,6 +311,79 @@ def test_append_gather(m, dtype, D, P, KVH, G, q_len, kv_len, pad, layout, rot):
         assert (ko[n:] == 5.0).all() and (vo[n:] == 5.0).all()
 
 
+@pytest.mark.parametrize("layout,rot", [("none", 0), ("pairs", 64), ("halves", 64), ("halves", 22)])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_append_gather_odd_offsets(m, dtype, layout, rot):
+    """rows that are not 16-byte aligned, queries turned in place: the aligned call's bits"""
+    D, KVH, H, dt = 64, 3, 6, TYPES[dtype]
+    q_len, kv_len = [5, 1, 37], [9, 70, 37]
+    a, b = (Case(m, q_len, kv_len, KVH, D, 16, pad=2, fill=None) for _ in range(2))
+    x = rand(5, a.T, H + 2 * KVH, D, dtype=dt).cuda()
+    wide = torch.full((a.T, (H + 2 * KVH) * D + 5), 5.0, dtype=dt, device="cuda")
+    odd = wide[:, 3:-2].unflatten(1, (H + 2 * KVH, D))
+    odd.copy_(x)
+    r = m.Rope(rot, 1e4, 512, m.ROPE_PAIRS if layout == "pairs" else m.ROPE_HALVES) if rot else None
+    qo = x[:, :H].clone()
+    for c, y, o in ((a, x, qo), (b, odd, odd[:, :H])):
+        c.cache.append(c.batch, rows(m, y[:, H:H + KVH]), rows(m, y[:, H + KVH:]), rope=r,
+                       q=rows(m, y[:, :H]), q_out=rows(m, o), stream=LEGACY)
+        assert c.cache.status() == 0
+    assert torch.equal(a.pages, b.pages) and torch.equal(odd[:, :H], qo)
+    assert torch.equal(odd[:, H:], x[:, H:]) and (wide[:, :3] == 5.0).all() and (wide[:, -2:] == 5.0).all()
+    ko, vo = x[:, H:H + KVH].clone(), x[:, H + KVH:].clone()
+    a.cache.gather(a.batch, rows(m, ko), rows(m, vo), stream=LEGACY)
+    b.cache.gather(b.batch, rows(m, odd[:, H:H + KVH]), rows(m, odd[:, H + KVH:]), stream=LEGACY)
+    assert torch.equal(odd[:, H:H + KVH], ko) and torch.equal(odd[:, H + KVH:], vo)
+
+
+@pytest.mark.parametrize("layout", ["pairs", "halves"])
+@pytest.mark.parametrize("T,D,KVH", [(2500, 64, 2), (6001, 128, 1), (20001, 64, 1)])
+def test_append_gather_many_tokens(m, T, D, KVH, layout):
+    """tokens enough that a CTA takes 2, 4, 8 .. of them, ragged sequences inside them: the
+    bytes of a call a sequence"""
+    rng = np.random.default_rng(T)
+    q_len = [1, 0, 1, 700, 3, 33]
+    q_len = [int(x) for x in q_len + [T - sum(q_len)]]
+    before = [int(x) for x in rng.integers(0, 90, len(q_len))]
+    kv_len = [x + y for x, y in zip(q_len, before)]
+    P, H = 64, KVH
+    need = [-(-x // P) for x in kv_len]
+    perm = rng.permutation(sum(need))
+    table = np.full((len(kv_len), max(need)), -1, np.int32)
+    at = 0
+    for i, n in enumerate(need):
+        table[i, :n] = perm[at:at + n]
+        at += n
+    start = np.concatenate([[0], np.cumsum(q_len)])
+    dev = [cuda_i32(start), cuda_i32(kv_len), torch.tensor(table, device="cuda")]
+    x = rand(1, T, H + 2 * KVH, D, dtype=torch.bfloat16).cuda()
+    r = m.Rope(D, 1e4, 32768, m.ROPE_PAIRS if layout == "pairs" else m.ROPE_HALVES)
+    got = []
+    for whole in (True, False):
+        cache = m.KVCache(sum(need), P, KVH, D)
+        out = torch.full((T, H + 2 * KVH, D), 5.0, dtype=x.dtype, device="cuda")
+        for i in [None] if whole else [j for j in range(len(q_len)) if q_len[j]]:
+            a, n = (0, T) if whole else (int(start[i]), q_len[i])
+            one = dev if whole else [cuda_i32([0, n]), dev[1][i:], dev[2][i:]]
+            batch = m.KVBatch(len(q_len) if whole else 1, n, max(q_len), max(kv_len),
+                              *[y.data_ptr() for y in one], table.shape[1])
+            y, o = x[a:a + n], out[a:a + n]
+            cache.append(batch, rows(m, y[:, H:H + KVH]), rows(m, y[:, H + KVH:]), rope=r,
+                         q=rows(m, y[:, :H]), q_out=rows(m, o[:, :H]), stream=LEGACY)
+            cache.gather(batch, rows(m, o[:, H:H + KVH]), rows(m, o[:, H + KVH:]), stream=LEGACY)
+        assert cache.status() == 0
+        got.append(out)
+    assert torch.equal(*got)
+    # and the values themselves, the keys after the rotation
+    pos = torch.cat([torch.arange(b, b + n) for b, n in zip(before, q_len)])
+    p, kt = cuda_i32(pos.tolist()), x[:, H:H + KVH].float().contiguous()
+    r.forward(T, D, p.data_ptr(), rows(m, kt), rows(m, kt), stream=LEGACY)
+    for i, want in ((H, kt), (H + KVH, x[:, H + KVH:].float())):
+        want = want.cpu().numpy()
+        y = torch.tensor(ref.values(*ref.quantize(want))).to(torch.bfloat16)
+        assert torch.equal(got[0][:, i:i + KVH].cpu(), y)
+
+
 def test_quantizer_edges(m):
     """scales at both ends of fp16, ties of the largest magnitude, rounding to even, a
     block with an infinity"""
@@ -394,6 +493,24 @@ def test_attention_strides_scale_no_lse(m):
             c.check(q, o, lse, scale=scale)
             o2, l2 = c.attend(q, scale=scale, lse=False)
             assert torch.equal(o2, o) and (l2 == 6.0).all()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_attention_in_place_shared_pages(m, dtype):
+    """results over their queries; two sequences that hold the same pages"""
+    D, KVH, G = 128, 2, 4
+    c = Case(m, [1, 1, 40, 1], [700, 700, 90, 0], KVH, D, 32, pad=2)
+    c.table[1] = c.table[0]
+    c.k[1], c.v[1] = c.k[0], c.v[0]
+    c.dev[2].copy_(torch.tensor(c.table))
+    q = rand(9, c.T, KVH * G, D, dtype=TYPES[dtype]).cuda()
+    q[c.start[-1]:] = 5.0
+    out, lse = c.attend(q)
+    same = q.clone()
+    same, lse2 = c.attend(same, out=same)
+    assert c.cache.status() == 0
+    c.check(q, out, lse)
+    assert torch.equal(same, out) and torch.equal(lse, lse2)
 
 
 def test_attention_extreme_values(m):
