@@ -15,22 +15,29 @@
 // With the cache as the 16-row operand a decode step's few queries (the heads
 // of a KV head's group) fill 8 columns instead of 16 rows, and the codes go
 // from shared memory to operand registers without a transposition: the page
-// layout places a thread's nibbles of all blocks side by side.  S^T comes out
-// with a row per lane group and P^T wants a column per lane group: one
-// movmatrix per 8 x 8 tile turns it.
+// layout places a thread's nibbles of all blocks side by side, and a nibble
+// masked out in place is an fp16 subnormal.  S^T comes out with a row per lane
+// group and P^T wants a column per lane group: one movmatrix per 8 x 8 tile
+// turns it.
 //
 // fp16 weights: p <= 16 (the running maximum may lag by 4, in exponents of 2;
-// then nothing needs rescaling), times 2^10, times the row's V scale brought to
-// [1, 2) by a power of two per block, so weights down to 2^-24 of the largest
-// keep fp16's full precision.  q is brought to 2^13 by a power of two per row.
-// fp32 rows take two columns, the fp16 value and the fp16 remainder.
+// then nothing needs rescaling), times 2^10, times the row's V scale brought below
+// 2 by a power of two per block (the block's largest so far to [1, 2), which leaves
+// fp16's range to the others), so weights down to 2^-24 of the largest keep fp16's
+// full precision where their block's V scale is near its largest.  A weight of 16-bit
+// rows is rounded to fp16 and its product with the scale once more: 2^-10 in all,
+// below what rounding the output to bf16 costs and twice fp16's; fp32 rows take two
+// columns, the fp16 value of the fp32 product and the fp16 remainder.  q is brought
+// to 2^13 by a power of two per row, so that fp16 holds 16-bit rows' values exactly
+// unless they are 2^-27 of the row's largest.
 //
 // Work: an item is a KV head of a sequence, a tile of its query rows (query
-// token x head of the group) and a run of 32-row key tiles; the CTA's 4 warps
-// take the run's tiles in turn, each with a ring of asynchronous copies of its
-// own, and join their sums at the end.  The run's length is chosen on the device from
-// the batch's lengths so that the items fill the GPU however ragged they are;
-// a tile of queries with several runs is joined by a second kernel.
+// token x head of the group) and a run of 32-row key tiles, and an item is a warp's:
+// the 4 warps of a CTA share nothing, so nothing waits.  (4 warps that took an item's
+// tiles in turn and joined their sums in shared memory: 47 us instead of 39 for 64
+// sequences, 243 instead of 195 for a prompt.)  The run's length is chosen on the
+// device from the batch's lengths so that the items fill the GPU however ragged they
+// are; a tile of queries with several runs is joined by a second kernel.
 #include "kv.cuh"
 
 #include <type_traits>
@@ -40,10 +47,10 @@ namespace {
 
 constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps;
 constexpr int kAttnTile = 32;      // key rows of a warp's copy
-constexpr int kAttnStages = 3;     // copies in a warp's ring
-constexpr int kRunMin = 1;         // tiles of a run
-constexpr int kRunMax = 256;       // 512 products in one fp32 chain
-constexpr float kLag = 4.0f;       // exponents of 2 that the running maximum may lag
+constexpr int kAttnStages = 2;     // copies in a warp's ring (3: 39.4 us for 64 sequences, 36.7 with 2)
+constexpr int kRunMin = 1;         // tiles of a run at least
+constexpr int kRunMax = 256;       // where runs are joined: 512 products in one fp32 chain
+constexpr float kLag = 4.0f;       // exponents of 2 that the running maximum may lag (0: prompt 226 us, 196)
 constexpr float kLift = 10.0f;     // weights are held times 2^10
 constexpr float kNoMax = 3.0e38f;  // the bias kLift - m before any row was seen
 
@@ -133,7 +140,8 @@ __device__ __forceinline__ int warp_scan(int v)
 // plan from the lengths, 32 sequences at a time: all work in key tiles over the
 // items wanted gives the run's length (in fp32: any length is right); sums over the
 // sequences before give a sequence's first item.  The sums fit 32 bits where the
-// arrays keep to the call's bounds (the host checks those).
+// arrays keep to the call's bounds (the host checks those); where q_start does not,
+// they may not, and no item is taken that lies outside its sequence.
 template <int RPT, bool ITEM>
 __device__ __forceinline__ bool find_item(const AttnArgs &a, int index, Item &f)
 {
@@ -184,6 +192,8 @@ __device__ __forceinline__ bool find_item(const AttnArgs &a, int index, Item &f)
 			const unsigned rest = a.by_kvh.div(at);
 			f.kvh = at - rest * a.KVH;
 			const unsigned rank = ITEM ? rest / (unsigned)runs : rest;
+			if (rank >= (unsigned)tiles)   // sums that do not fit (see above)
+				return false;
 			f.run = ITEM ? rest - rank * (unsigned)runs : 0;
 			f.first = i0 + rank * runs * a.KVH + f.kvh;
 			f.tile = tiles - 1 - (int)rank;
@@ -318,8 +328,9 @@ __device__ __forceinline__ uint32_t codes_high(uint32_t w)
 }
 constexpr float kCodeUnit = 16777216.0f;   // 2^24
 
-// tile row of A's row j: rows j and j ^ 2.. stay within 16; chosen so that the
-// 8 rows of a shared-memory read touch both halves of the banks
+// The tile row that stands as row j of A (of 8): any order will do that K and V, and
+// so S^T and P^T, share.  This one lets the 8 rows that a shared-memory read takes
+// together begin in banks of their own.
 __device__ __forceinline__ int tile_row(int j) { return j ^ ((j >> 1) & 1); }
 
 // NW 32-bit words from shared memory
@@ -393,11 +404,15 @@ struct StageLayout {
 template <int HL>
 constexpr int kAttnSmem = kAttnWarps * kAttnStages * StageLayout<HL>::kBytes;
 
-#ifndef ATTN_MINB
-#define ATTN_MINB (HL == 128 && NT == 1 ? 4 : 1)
-#endif
+// queries as operands in registers, or in shared memory where there are more of them
+// than registers (128 a lane at HL * NT = 512)
 template <int HL, int NT>
 constexpr bool kQInRegs = HL * NT <= 256;
+
+// CTAs of an SM that the registers are cut for: 4 where 128 a lane do (HL 128, one
+// column tile: 4 sequences of 131072 rows 126 us, left to itself 141; 3: 143).
+template <int HL, int NT>
+constexpr int kAttnCtas = HL == 128 && NT == 1 ? 4 : 1;
 
 // 16 bytes to shared memory, in flight until its group is waited for
 __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t *src)
@@ -412,8 +427,12 @@ __device__ __forceinline__ void copies_wait()
 	asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// grid: the plan's items, kAttnWarps to a CTA.  Few queries (4 sequences of 131072 rows,
+// 32 heads on 8: 526 MB in 124 us, 4.25 TB/s of 6.5) are bound by the instructions
+// that take codes apart, a batch of 64 such sequences of up to 4096 rows (72 MB in
+// 37 us) by latency: a few tiles a warp between its plan and its last store.
 template <typename T, int HL, int NT>
-__global__ void __launch_bounds__(kAttnThreads, ATTN_MINB) kv_attn_kernel(AttnArgs a)
+__global__ void __launch_bounds__(kAttnThreads, kAttnCtas<HL, NT>) kv_attn_kernel(AttnArgs a)
 {
 	constexpr bool SPLIT = sizeof(T) == 4;        // two columns a row
 	constexpr int RPN = SPLIT ? 4 : 8;            // rows of an 8-column tile
@@ -973,9 +992,10 @@ __global__ void __launch_bounds__(kAttnThreads, ATTN_MINB) kv_attn_kernel(AttnAr
 	}
 }
 
-// The runs of a tile's query rows joined, a CTA a tile or some rows of it: each
-// row by as many of its warps as the rows leave it, which take the runs in turn.  A few dependent loads
-// long, so the sums of a warp's first runs leave before the factors are known.
+// The runs of a tile's query rows joined, a CTA a tile or some rows of it: each row by
+// as many of its warps as the rows leave it, which take the runs in turn.  A few
+// dependent loads long, so the sums of a warp's first runs leave before the factors
+// are known (latency: 2 to 5 us behind the kernel above).
 constexpr int kMergeWarps = 4;
 template <typename T, int HL, int RPT>
 __global__ void __launch_bounds__(32 * kMergeWarps) kv_merge_kernel(AttnArgs a)
@@ -1102,7 +1122,9 @@ Plan plan_of(const moe_kv_cache *c, const moe_kv_batch *b, int64_t H, bool fp32)
 	const int64_t HL = c->d.head_len, KVH = c->d.n_kv_heads, G = H / KVH;
 	const int64_t rows = b->max_q * G;   // query rows of a sequence's KV head
 	const int per = fp32 ? 4 : 8;
-	// as few columns as hold the rows; many rows: as many as registers hold
+	// as few columns as hold the rows (4 tiles for a decode batch's 4 rows: 82 us
+	// instead of 39); many rows: as many as registers hold (a prompt with 2: 216,
+	// with 4: 196)
 	p.nt = rows <= per ? 1 : rows <= 2 * per || HL == 256 ? 2 : 4;
 	p.rpt = per * p.nt;
 	const int64_t by_seq = b->n_seqs * ((rows + p.rpt - 1) / p.rpt);
@@ -1110,7 +1132,9 @@ Plan plan_of(const moe_kv_cache *c, const moe_kv_batch *b, int64_t H, bool fp32)
 	p.tiles = KVH * (by_seq < by_token ? by_seq : by_token);
 	p.rows = (int)(rows < p.rpt ? rows : p.rpt);
 	// items for whole waves of resident warps (16 an SM, fewer for wide tiles), the
-	// runs' remainders among them (a remainder a query tile at most)
+	// runs' remainders among them (a remainder a query tile at most; left out of the
+	// count: 41.4 us for 64 sequences, 39.3).  Two waves: 46, and 142 instead of 126
+	// for 4 x 131072 rows
 	const int64_t wave = (int64_t)sm_count() * kAttnWarps * (HL * p.nt <= 128 ? 4 : 2);
 	int64_t want = wave - p.tiles;
 	while (want < wave / 2)
@@ -1144,7 +1168,8 @@ cudaError_t launch_attn_as(const AttnArgs &a, const Plan &p, cudaStream_t st)
 	if (!p.split)
 		return cudaSuccess;
 	cudaLaunchConfig_t cfg{};
-	// few tiles: their rows over several CTAs, up to one a row
+	// few tiles: their rows over several CTAs, up to one a row (one CTA a tile: 8
+	// drafted tokens 39 us, 23; 4 x 131072 rows 137, 126)
 	const int64_t y = 8 * (int64_t)sm_count() / p.tiles;
 	cfg.gridDim = dim3((unsigned)p.tiles, (unsigned)(y < 1 ? 1 : y < p.rows ? y : p.rows));
 	cfg.blockDim = dim3(32 * kMergeWarps);
