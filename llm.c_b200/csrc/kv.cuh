@@ -40,7 +40,7 @@ namespace moe {
 constexpr int kRopeLow = 1024;   // rows of the low table
 
 // bits of a handle's error word
-enum { kKvErrBatch = 1, kKvErrPage = 2, kKvErrPos = 4 };
+enum { kKvErrBatch = 1, kKvErrPage = 2, kKvErrPos = 4, kKvErrWait = 8 };
 
 // ---------------------------------------------------------------- host side
 inline int kv_fail(int code, const char *fmt, ...)

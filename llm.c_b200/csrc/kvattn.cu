@@ -38,204 +38,17 @@
 // sequences, 243 instead of 195 for a prompt.)  The run's length is chosen on the
 // device from the batch's lengths so that the items fill the GPU however ragged they
 // are; a tile of queries with several runs is joined by a second kernel.
-#include "kv.cuh"
+#include "kvattn.cuh"
 
 #include <type_traits>
 
 namespace moe {
+using namespace kva;
 namespace {
 
 constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps;
-constexpr int kAttnTile = 32;      // key rows of a warp's copy
+constexpr int kWideMin = 128;      // query rows of a sequence's KV head for kvwide.cu's kernel
 constexpr int kAttnStages = 2;     // copies in a warp's ring (3: 39.4 us for 64 sequences, 36.7 with 2)
-constexpr int kRunMin = 1;         // tiles of a run at least
-constexpr int kRunMax = 256;       // where runs are joined: 512 products in one fp32 chain
-constexpr float kLag = 4.0f;       // exponents of 2 that the running maximum may lag (0: prompt 226 us, 196)
-constexpr float kLift = 10.0f;     // weights are held times 2^10
-constexpr float kNoMax = 3.0e38f;  // the bias kLift - m before any row was seen
-
-// j / n and j % n for any 31-bit j: the quotient by a rounded-down reciprocal is at
-// most one short.  (A division by a runtime value is some twenty dependent
-// instructions, which a decode step's few warps wait for.)
-struct QuickDiv {
-	unsigned n = 1, m = 0;
-	QuickDiv() {}
-	explicit QuickDiv(unsigned n_) : n(n_), m(n_ > 1 ? (unsigned)(0x100000000ull / n_) : 0) {}
-	__device__ __forceinline__ int div(int j) const
-	{
-		if (n == 1)
-			return j;
-		const unsigned q = __umulhi((unsigned)j, m);
-		return (int)(q + ((unsigned)j - q * n >= n));
-	}
-};
-
-struct AttnArgs {
-	BatchArgs b;
-	const void *q;
-	void *out;
-	int64_t q_ts, q_hs, o_ts, o_hs;
-	float *lse;
-	const uint8_t *pages;
-	int64_t page_bytes;
-	int H, KVH, G;
-	QuickDiv by_g, by_kvh;
-	int causal, window;
-	float scale2;        // scale * log2 e
-	int q_vec, o_vec;    // 16-byte aligned rows
-	int target;          // items wanted (0: one run a tile)
-	int64_t items;       // items that the workspace holds
-	float *part;         // [item][row][HL + 4]: sums, bias, weights' sum
-	int part_rows;       // rows of an item that can be in use
-};
-
-// one item of the batch
-struct Item {
-	int b, kvh, tile;    // sequence, KV head, tile of query rows
-	int s0, n, kv;       // its first token, queries, cache rows
-	int r0, rows;        // first query row (token * G + head) and rows of the tile
-	int lo, hi;          // cache rows that the tile sees
-	int t0, t1;          // the item's key tiles
-	int run, runs;       // which run of how many
-	int first;           // index of the tile's first item
-};
-
-__device__ __forceinline__ bool seq_of(const AttnArgs &a, int b, int &s0, int &n, int &kv)
-{
-	s0 = a.b.q_start[b];
-	const int s1 = a.b.q_start[b + 1];
-	n = s1 - s0;
-	kv = a.b.kv_len[b];
-	const bool ok = s0 >= 0 && s1 >= s0 && s1 <= a.b.T && n <= a.b.max_q && kv >= 0 &&
-			kv <= a.b.max_kv && (b > 0 || s0 == 0);
-	if (!ok) {
-		n = 0;
-		if (blockIdx.x == 0 && threadIdx.x < 32)
-			atomicOr(a.b.err, kKvErrBatch);
-	}
-	return ok;
-}
-
-// key tiles of a sequence, over all of its queries
-__device__ __forceinline__ int seq_tiles(const AttnArgs &a, int n, int kv)
-{
-	const int lo = a.window ? max(0, kv - n - a.window + 1) : 0;
-	return (kv + kAttnTile - 1) / kAttnTile - lo / kAttnTile;
-}
-
-// sums of v over the lanes up to this one
-__device__ __forceinline__ int warp_scan(int v)
-{
-	const int lane = threadIdx.x % 32;
-#pragma unroll
-	for (int o = 1; o < 32; o *= 2) {
-		const int w = __shfl_up_sync(0xffffffffu, v, o);
-		v += lane >= o ? w : 0;
-	}
-	return v;
-}
-
-// Item `index` of the batch (ITEM), or tile `index` of its query tiles with the
-// tile's number of runs, by one warp.  Every CTA of both kernels derives the same
-// plan from the lengths, 32 sequences at a time: all work in key tiles over the
-// items wanted gives the run's length (in fp32: any length is right); sums over the
-// sequences before give a sequence's first item.  The sums fit 32 bits where the
-// arrays keep to the call's bounds (the host checks those); where q_start does not,
-// they may not, and no item is taken that lies outside its sequence.
-template <int RPT, bool ITEM>
-__device__ __forceinline__ bool find_item(const AttnArgs &a, int index, Item &f)
-{
-	const int lane = threadIdx.x % 32, B = a.b.B;
-	int s0 = 0, n = 0, kv = 0;
-	int run = 1 << 30;   // target 0: query tiles enough, one run each
-	if (a.target) {
-		float all = 0.0f;
-		for (int b = lane; b < B; b += 32)
-			if (seq_of(a, b, s0, n, kv))
-				all += (float)((n * a.G + RPT - 1) / RPT) * (float)seq_tiles(a, n, kv);
-		run = (int)fminf(ceilf(warp_sum(all) * a.KVH / a.target), (float)kRunMax);
-		run = max(run, kRunMin);
-	}
-	int item0 = 0, tile0 = 0;
-	for (int b0 = 0; b0 < B; b0 += 32) {
-		const int b = b0 + lane;
-		int tiles = 0, runs = 0;
-		if (B > 32 || !a.target) {
-			n = 0;
-			if (b < B)
-				seq_of(a, b, s0, n, kv);
-		}
-		if (b < B && n > 0) {
-			tiles = (n * a.G + RPT - 1) / RPT;
-			runs = max(1, (int)((unsigned)(seq_tiles(a, n, kv) + run - 1) / (unsigned)run));
-		}
-		const int items = tiles * runs * a.KVH;
-		const int iend = item0 + warp_scan(items);
-		const int tend = ITEM ? iend : tile0 + warp_scan(tiles * a.KVH);
-		const unsigned m = __ballot_sync(0xffffffffu, index < (ITEM ? iend : tend));
-		if (m) {
-			// the first sequence that ends behind it
-			const int src = __ffs(m) - 1;
-			s0 = __shfl_sync(0xffffffffu, s0, src);
-			n = __shfl_sync(0xffffffffu, n, src);
-			kv = __shfl_sync(0xffffffffu, kv, src);
-			tiles = __shfl_sync(0xffffffffu, tiles, src);
-			runs = __shfl_sync(0xffffffffu, runs, src);
-			const int i0 = __shfl_sync(0xffffffffu, iend - items, src);
-			const int t0 = __shfl_sync(0xffffffffu, tend - tiles * a.KVH, src);
-			const unsigned at = index - (ITEM ? i0 : t0);
-			// KV heads side by side; the last tiles, which see the most, first
-			f.b = b0 + src;
-			f.s0 = s0;
-			f.n = n;
-			f.kv = kv;
-			const unsigned rest = a.by_kvh.div(at);
-			f.kvh = at - rest * a.KVH;
-			const unsigned rank = ITEM ? rest / (unsigned)runs : rest;
-			if (rank >= (unsigned)tiles)   // sums that do not fit (see above)
-				return false;
-			f.run = ITEM ? rest - rank * (unsigned)runs : 0;
-			f.first = i0 + rank * runs * a.KVH + f.kvh;
-			f.tile = tiles - 1 - (int)rank;
-			f.r0 = f.tile * RPT;
-			f.rows = min(RPT, n * a.G - f.r0);
-			const int p0 = kv - n + a.by_g.div(f.r0), p1 = kv - n + a.by_g.div(f.r0 + f.rows - 1);
-			f.lo = a.window ? max(0, p0 - a.window + 1) : 0;
-			f.hi = a.causal ? min(kv, p1 + 1) : kv;
-			const int ta = f.lo / kAttnTile, tb = max(ta, (f.hi + kAttnTile - 1) / kAttnTile);
-			f.runs = max(1, (int)((unsigned)(tb - ta + run - 1) / (unsigned)run));
-			f.t0 = min(tb, ta + f.run * run);
-			f.t1 = min(tb, f.t0 + run);
-			// q_start that does not rise can name more items than it has
-			// tokens for: those behind the plan's bound are left out
-			return f.first >= 0 && f.first + (int64_t)(runs - 1) * a.KVH < a.items &&
-			       (!ITEM || f.run < f.runs);
-		}
-		item0 = __shfl_sync(0xffffffffu, iend, 31);
-		tile0 = __shfl_sync(0xffffffffu, tend, 31);
-	}
-	return false;
-}
-
-// found by the CTA's first warp for all of them
-template <int RPT, bool ITEM>
-__device__ __forceinline__ bool cta_item(const AttnArgs &a, int index, Item &f)
-{
-	__shared__ Item found;
-	__shared__ int ok;
-	if (threadIdx.x < 32) {
-		Item x;
-		const bool in = find_item<RPT, ITEM>(a, index, x);
-		if (threadIdx.x == 0) {
-			found = x;
-			ok = in;
-		}
-	}
-	__syncthreads();
-	f = found;
-	return ok;
-}
-
 __device__ __forceinline__ void mma_step(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
 					 uint32_t b1)
 {
@@ -270,33 +83,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
 	uint32_t y;
 	asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
 	return y;
-}
-
-__device__ __forceinline__ float ex2(float x)
-{
-	float y;
-	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-	return y;
-}
-
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
-__device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
-__device__ __forceinline__ uint32_t pack_h2(float lo, float hi)
-{
-	return h2_bits(__floats2half2_rn(lo, hi));
-}
-
-// half `at` of a word
-__device__ __forceinline__ float half_of(uint32_t w, int at)
-{
-	const __half2 h = bits_h2(w);
-	return at ? __high2float(h) : __low2float(h);
-}
-
-__device__ __forceinline__ uint32_t set_half(uint32_t w, int at, float v)
-{
-	const uint32_t h = __half_as_ushort(__float2half_rn(v));
-	return at ? (w & 0xffffu) | h << 16 : (w & 0xffff0000u) | h;
 }
 
 // half `at` of a word, twice
@@ -355,44 +141,6 @@ __device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[NW])
 	}
 }
 
-// Row r of a tile as it leaves: sums over the weights' sum, zeros where nothing was
-// seen, and its log-sum-exp
-template <typename T>
-struct RowOut {
-	T *p;
-	float *lse_at;
-	float il, l, bias;
-	bool vec;
-	__device__ __forceinline__ RowOut(const AttnArgs &a, const Item &it, int r, float bias_, float l_)
-		: il(l_ == 0.0f ? 0.0f : 1.0f / l_), l(l_), bias(bias_), vec(a.o_vec)
-	{
-		const int qr = it.r0 + r, i = a.by_g.div(qr);
-		const int token = it.s0 + i, head = it.kvh * a.G + qr - i * a.G;
-		p = static_cast<T *>(a.out) + token * a.o_ts + head * a.o_hs;
-		lse_at = a.lse ? a.lse + (int64_t)token * a.H + head : nullptr;
-	}
-	__device__ __forceinline__ void two(int e, float x, float y) const
-	{
-		x *= il;
-		y *= il;
-		if (!vec) {
-			p[e] = from_f32<T>(x);
-			p[e + 1] = from_f32<T>(y);
-		} else if constexpr (sizeof(T) == 4) {
-			*reinterpret_cast<float2 *>(p + e) = make_float2(x, y);
-		} else {
-			T v[2] = {from_f32<T>(x), from_f32<T>(y)};
-			*reinterpret_cast<uint32_t *>(p + e) = *reinterpret_cast<uint32_t *>(v);
-		}
-	}
-	__device__ __forceinline__ void lse() const
-	{
-		if (lse_at)
-			*lse_at = l == 0.0f ? -__int_as_float(0x7f800000)
-					    : 0.693147180559945f * (log2f(l) - bias);
-	}
-};
-
 template <int HL>
 struct StageLayout {
 	static constexpr int NB = HL / 32;
@@ -413,19 +161,6 @@ constexpr bool kQInRegs = HL * NT <= 256;
 // column tile: 4 sequences of 131072 rows 126 us, left to itself 141; 3: 143).
 template <int HL, int NT>
 constexpr int kAttnCtas = HL == 128 && NT == 1 ? 4 : 1;
-
-// 16 bytes to shared memory, in flight until its group is waited for
-__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t *src)
-{
-	asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// all but the newest N groups have landed
-template <int N>
-__device__ __forceinline__ void copies_wait()
-{
-	asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 
 // grid: the plan's items, kAttnWarps to a CTA.  Few queries (4 sequences of 131072 rows,
 // 32 heads on 8: 526 MB in 124 us, 4.25 TB/s of 6.5) are bound by the instructions
@@ -992,150 +727,20 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas<HL, NT>) kv_attn_kerne
 	}
 }
 
-// The runs of a tile's query rows joined, a CTA a tile or some rows of it: each row by
-// as many of its warps as the rows leave it, which take the runs in turn.  A few
-// dependent loads long, so the sums of a warp's first runs leave before the factors
-// are known (latency: 2 to 5 us behind the kernel above).
-constexpr int kMergeWarps = 4;
-template <typename T, int HL, int RPT>
-__global__ void __launch_bounds__(32 * kMergeWarps) kv_merge_kernel(AttnArgs a)
-{
-	constexpr int OS = HL + 4, E4 = HL / 4;                  // float4s of a row
-	constexpr int W = E4 < 32 ? E4 : 32, SIDE = 32 / W, NV = E4 / W;
-	constexpr int BATCH = 4;
-	__shared__ float4 red[kMergeWarps][E4];
-	Item it;
-	const bool mine = cta_item<RPT, false>(a, blockIdx.x, it) && it.runs > 1;
-	griddep_wait();   // the runs are written
-	if (!mine)
-		return;
-	const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-	// the CTA's rows of the tile; warps of a row
-	const int each = (a.part_rows + gridDim.y - 1) / gridDim.y;
-	const int from = blockIdx.y * each, to = min(from + each, it.rows);
-	int share = kMergeWarps;
-	while (share > 1 && share * (to - from) > kMergeWarps)
-		share /= 2;
-	const int part = warp % share, ds = share * SIDE;
-	const int64_t step = (int64_t)a.KVH * a.part_rows * OS;   // between the runs of a tile
-	for (int r0 = from; r0 < to; r0 += kMergeWarps / share) {
-		const int r = r0 + warp / share;
-		const bool row = r < to;   // the whole warp
-		const float *pp = a.part + ((int64_t)it.first * a.part_rows + (row ? r : 0)) * OS;
-		const int s0 = part * SIDE + lane / W, e = lane % W * 4;
-		const int runs = row ? it.runs : 0;
-		float4 x[BATCH][NV], o[NV];
-		float xb[BATCH];
-		auto load = [&](int s) {
-#pragma unroll
-			for (int k = 0; k < BATCH; k++) {
-				const float *p = pp + (s + k * ds) * step;
-				const bool in = s + k * ds < runs;
-				xb[k] = in ? p[HL] : kNoMax;
-#pragma unroll
-				for (int v = 0; v < NV; v++)
-					x[k][v] = in ? *reinterpret_cast<const float4 *>(p + e + 4 * W * v)
-						     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-			}
-		};
-		load(s0);
-		float b = kNoMax, l = 0.0f;
-		for (int s = lane; s < runs; s += 32)
-			b = fminf(b, pp[s * step + HL]);
-		b = -warp_max(-b);
-		for (int s = lane; s < runs; s += 32)
-			l += pp[s * step + HL + 1] * ex2(b - pp[s * step + HL]);
-		l = warp_sum(l);
-#pragma unroll
-		for (int v = 0; v < NV; v++)
-			o[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-		for (int s = s0;;) {
-#pragma unroll
-			for (int k = 0; k < BATCH; k++) {
-				const float f = ex2(b - xb[k]);
-#pragma unroll
-				for (int v = 0; v < NV; v++) {
-					o[v].x = fmaf(x[k][v].x, f, o[v].x);
-					o[v].y = fmaf(x[k][v].y, f, o[v].y);
-					o[v].z = fmaf(x[k][v].z, f, o[v].z);
-					o[v].w = fmaf(x[k][v].w, f, o[v].w);
-				}
-			}
-			s += BATCH * ds;
-			if (s - lane / W >= runs)
-				break;
-			load(s);
-		}
-#pragma unroll
-		for (int v = 0; v < NV; v++) {
-			if (SIDE == 2) {
-				o[v].x += __shfl_xor_sync(0xffffffffu, o[v].x, 16);
-				o[v].y += __shfl_xor_sync(0xffffffffu, o[v].y, 16);
-				o[v].z += __shfl_xor_sync(0xffffffffu, o[v].z, 16);
-				o[v].w += __shfl_xor_sync(0xffffffffu, o[v].w, 16);
-			}
-			if (share > 1 && lane < W)
-				red[warp][lane + W * v] = o[v];
-		}
-		if (share > 1) {   // one round of rows then: share * rows <= the warps
-			__syncthreads();
-			if (part == 0 && lane < W) {
-#pragma unroll
-				for (int v = 0; v < NV; v++)
-					for (int w = 1; w < share; w++) {
-						const float4 y = red[warp + w][lane + W * v];
-						o[v].x += y.x;
-						o[v].y += y.y;
-						o[v].z += y.z;
-						o[v].w += y.w;
-					}
-			}
-		}
-		if (row && part == 0 && lane < W) {
-			const RowOut<T> out(a, it, r, b, l);
-#pragma unroll
-			for (int v = 0; v < NV; v++) {
-				out.two(e + 4 * W * v, o[v].x, o[v].y);
-				out.two(e + 4 * W * v + 2, o[v].z, o[v].w);
-			}
-			if (lane == 0)
-				out.lse();
-		}
-	}
-}
-
 // ---------------------------------------------------------------- launches
-// the sizes that a launch is planned with, from the call's bounds alone
-struct Plan {
-	int nt = 1, rpt = 8;     // column tiles, query rows of an item
-	int rows = 8;            // rows of them that can be in use
-	int64_t tiles = 0;       // at most so many query tiles x KV heads
-	int64_t items = 0;       // and items
-	int target = 0;
-	bool split = false;      // runs at all
-	size_t part_bytes = 0;
-};
-
-Plan plan_of(const moe_kv_cache *c, const moe_kv_batch *b, int64_t H, bool fp32)
+// `rows` is the most query rows of a sequence's KV head, p.rpt an item's and `wave` the
+// items that a GPU has at a time
+void plan_items(Plan &p, const moe_kv_cache *c, const moe_kv_batch *b, int64_t G, int64_t rows,
+		int64_t wave)
 {
-	Plan p;
-	const int64_t HL = c->d.head_len, KVH = c->d.n_kv_heads, G = H / KVH;
-	const int64_t rows = b->max_q * G;   // query rows of a sequence's KV head
-	const int per = fp32 ? 4 : 8;
-	// as few columns as hold the rows (4 tiles for a decode batch's 4 rows: 82 us
-	// instead of 39); many rows: as many as registers hold (a prompt with 2: 216,
-	// with 4: 196)
-	p.nt = rows <= per ? 1 : rows <= 2 * per || HL == 256 ? 2 : 4;
-	p.rpt = per * p.nt;
+	const int64_t KVH = c->d.n_kv_heads;
 	const int64_t by_seq = b->n_seqs * ((rows + p.rpt - 1) / p.rpt);
 	const int64_t by_token = b->n_tokens * G / p.rpt + b->n_seqs;
 	p.tiles = KVH * (by_seq < by_token ? by_seq : by_token);
 	p.rows = (int)(rows < p.rpt ? rows : p.rpt);
-	// items for whole waves of resident warps (16 an SM, fewer for wide tiles), the
-	// runs' remainders among them (a remainder a query tile at most; left out of the
-	// count: 41.4 us for 64 sequences, 39.3).  Two waves: 46, and 142 instead of 126
-	// for 4 x 131072 rows
-	const int64_t wave = (int64_t)sm_count() * kAttnWarps * (HL * p.nt <= 128 ? 4 : 2);
+	// items for whole waves, the runs' remainders among them (a remainder a query tile
+	// at most; left out of the count: 41.4 us for 64 sequences, 39.3).  Two waves: 46,
+	// and 142 instead of 126 for 4 x 131072 rows
 	int64_t want = wave - p.tiles;
 	while (want < wave / 2)
 		want += wave;
@@ -1149,9 +754,43 @@ Plan plan_of(const moe_kv_cache *c, const moe_kv_batch *b, int64_t H, bool fp32)
 		const int64_t most = p.tiles * ((longest + kRunMin - 1) / kRunMin);
 		p.items += 1 + (capped > p.target ? capped : p.target);
 		p.items = p.items < most ? p.items : most;
-		p.part_bytes = (size_t)(p.items * p.rows * (HL + 4) * 4);
+		p.part_bytes = (size_t)(p.items * p.rows * (c->d.head_len + 4) * 4);
 	}
-	return p;
+}
+
+// The kernels of a call: an item a warp (`narrow`), an item a CTA (`wide`), or both, each
+// for its sequences.  A wide item pays for kWideRows query rows whether they are there or
+// not: WIDE_NOTE.
+struct Plans {
+	bool narrow = false, wide = false;
+	Plan n, w;
+	size_t bytes() const { return n.part_bytes + w.part_bytes; }
+};
+
+Plans plan_of(const moe_kv_cache *c, const moe_kv_batch *b, int64_t H, bool fp32)
+{
+	Plans ps;
+	const int64_t HL = c->d.head_len, G = H / c->d.n_kv_heads;
+	const int64_t rows = b->max_q * G;   // query rows of a sequence's KV head
+	ps.wide = !fp32 && HL <= 128 && rows >= kWideMin;
+	// sequences of as many queries as the longest, or one
+	ps.narrow = !ps.wide || (b->n_seqs > 1 && b->n_tokens < b->n_seqs * b->max_q);
+	if (ps.narrow) {
+		const int64_t r = ps.wide ? kWideMin - 1 : rows;
+		const int per = fp32 ? 4 : 8;
+		// as few columns as hold the rows (4 tiles for a decode batch's 4 rows: 82 us
+		// instead of 39); many rows: as many as registers hold (a prompt with 2: 216,
+		// with 4: 196)
+		ps.n.nt = r <= per ? 1 : r <= 2 * per || HL == 256 ? 2 : 4;
+		ps.n.rpt = per * ps.n.nt;
+		// 16 resident warps an SM, fewer for wide tiles
+		plan_items(ps.n, c, b, G, r, (int64_t)sm_count() * kAttnWarps * (HL * ps.n.nt <= 128 ? 4 : 2));
+	}
+	if (ps.wide) {
+		ps.w.rpt = kWideRows;
+		plan_items(ps.w, c, b, G, rows, sm_count());
+	}
+	return ps;
 }
 
 template <typename T, int HL, int NT>
@@ -1165,21 +804,7 @@ cudaError_t launch_attn_as(const AttnArgs &a, const Plan &p, cudaStream_t st)
 		<<<(unsigned)((p.items + kAttnWarps - 1) / kAttnWarps), kAttnThreads, smem, st>>>(a);
 	if (cudaError_t e = cudaGetLastError())
 		return e;
-	if (!p.split)
-		return cudaSuccess;
-	cudaLaunchConfig_t cfg{};
-	// few tiles: their rows over several CTAs, up to one a row (one CTA a tile: 8
-	// drafted tokens 39 us, 23; 4 x 131072 rows 137, 126)
-	const int64_t y = 8 * (int64_t)sm_count() / p.tiles;
-	cfg.gridDim = dim3((unsigned)p.tiles, (unsigned)(y < 1 ? 1 : y < p.rows ? y : p.rows));
-	cfg.blockDim = dim3(32 * kMergeWarps);
-	cfg.stream = st;
-	cudaLaunchAttribute at[1];
-	at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-	at[0].val.programmaticStreamSerializationAllowed = 1;
-	cfg.attrs = at;
-	cfg.numAttrs = pdl_enabled() ? 1 : 0;
-	return cudaLaunchKernelEx(&cfg, kv_merge_kernel<T, HL, RPT>, a);
+	return launch_merge<T, HL, RPT>(a, p, st);
 }
 
 template <typename T>
@@ -1199,7 +824,7 @@ cudaError_t launch_attn(const AttnArgs &a, const Plan &p, int HL, cudaStream_t s
 // what a call may ask of its workspace: the same for every row type
 size_t workspace_of(const moe_kv_cache *c, const moe_kv_batch *b, int64_t H)
 {
-	const size_t x = plan_of(c, b, H, true).part_bytes, y = plan_of(c, b, H, false).part_bytes;
+	const size_t x = plan_of(c, b, H, true).bytes(), y = plan_of(c, b, H, false).bytes();
 	return x > y ? x : y;
 }
 
@@ -1267,8 +892,8 @@ int moe_kv_attention(moe_kv_cache *cache, const moe_kv_batch *batch, const moe_r
 		return rc;
 	DeviceGuard g(cache->device);
 	KV_CK(what, g.e);
-	const Plan p = plan_of(cache, batch, q->n_heads, q->type == MOE_F32);
-	if (p.items > 0x7fffffff || batch->max_q * (q->n_heads / KVH) > (1 << 30))
+	const Plans p = plan_of(cache, batch, q->n_heads, q->type == MOE_F32);
+	if (p.n.items > 0x7fffffff || p.w.items > 0x7fffffff || batch->max_q * (q->n_heads / KVH) > (1 << 30))
 		return kv_fail(MOE_ERR_INVALID, "%s: batch too large", what);
 	const size_t need = workspace_of(cache, batch, q->n_heads);
 	if (need && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need))
@@ -1295,13 +920,26 @@ int moe_kv_attention(moe_kv_cache *cache, const moe_kv_batch *batch, const moe_r
 	a.scale2 = scale * 1.44269504088896f;
 	a.q_vec = rows_vec16(q);
 	a.o_vec = rows_vec16(out);
-	a.target = p.split ? p.target : 0;
-	a.items = p.items;
-	a.part = static_cast<float *>(workspace);
-	a.part_rows = p.rows;
-	KV_CK(what, q->type == MOE_F32   ? launch_attn<float>(a, p, (int)D, st)
-		    : q->type == MOE_F16 ? launch_attn<__half>(a, p, (int)D, st)
-					 : launch_attn<__nv_bfloat16>(a, p, (int)D, st));
+	uint8_t *part = static_cast<uint8_t *>(workspace);
+	auto plan_args = [&](const Plan &x, int64_t least, int64_t most) {
+		a.target = x.split ? x.target : 0;
+		a.items = x.items;
+		a.part = reinterpret_cast<float *>(part);
+		a.part_rows = x.rows;
+		a.min_rows = (int)least;
+		a.max_rows = (int)most;
+		part += x.part_bytes;
+	};
+	if (p.wide) {   // first: its items take longest
+		plan_args(p.w, p.narrow ? kWideMin : 0, 1 << 30);
+		KV_CK(what, launch_wide(a, p.w, q->type, (int)D, st));
+	}
+	if (p.narrow) {
+		plan_args(p.n, 0, p.wide ? kWideMin - 1 : 1 << 30);
+		KV_CK(what, q->type == MOE_F32   ? launch_attn<float>(a, p.n, (int)D, st)
+			    : q->type == MOE_F16 ? launch_attn<__half>(a, p.n, (int)D, st)
+						 : launch_attn<__nv_bfloat16>(a, p.n, (int)D, st));
+	}
 	return MOE_OK;
 }
 

@@ -672,6 +672,8 @@ int moe_kv_status(moe_kv_cache *cache)
 		return MOE_OK;
 	KV_CK(what, cudaMemset(cache->err, 0, 4));
 	KV_CK(what, cudaDeviceSynchronize());   // before a call on any stream records the next
+	if (e & kKvErrWait)
+		return kv_fail(MOE_ERR_TIMEOUT, "%s: a bounded wait in the attention kernel expired", what);
 	return kv_fail(MOE_ERR_INVALID, "%s:%s%s%s", what,
 		       e & kKvErrBatch ? " q_start or kv_len out of range;" : "",
 		       e & kKvErrPage ? " page outside the cache;" : "",
