@@ -16,17 +16,20 @@
 // as kvattn.cu rounds (weight, then weight * scale).  They are brought below 2 by a power
 // of two a block, the largest so far to [1, 2).
 //
-// 18 warps: thread r of the first 256 has query row r and its softmax (two groups of 128,
-// whose TMEM lanes and columns are their own), 128 take K's codes apart and fetch the next
-// tile, 128 take V's apart, and a warp a group issues its products.  What waits for what:
+// 19 warps: thread r of the first 256 has query row r and its softmax (two groups of 128,
+// whose TMEM lanes and columns are their own), 128 take K's codes apart, 128 take V's
+// apart, a warp a group issues its products, and one fetches the tiles.  What waits for
+// what:
 //
-//   stagers  K of tile j: for the rows' reads of S of tile j - 2; V: for O += P V of tile
-//            j - 2 (K, V and the barriers are double)
+//   copier   tile j: for the stagers to be done with tile j - 4
+//   stagers  tile j there; its K: for S of tile j - 2; V: for O += P V of tile j - 2 (K, V
+//            and their barriers are double)
 //   issuer   S of tile i + 1 (double too): for its K and the rows' reads of S of tile
 //            i - 1, so it runs beside the softmax of tile i; then O += P V of tile i: for
 //            P and V
-//   rows     S of tile i to registers; softmax; O += P V of tile i - 1 done; P to
-//            shared memory
+//   rows     S of tile i to registers (and O += P V of tile i - 2, issued before it,
+//            done); softmax; P (double) to shared memory; where the maximum or V's
+//            factors move, O += P V of tile i - 1
 //
 // A barrier's next phase needs what follows a wait for this one, so none is missed.
 // All operands are rows of 64 bytes (32 values) in the 64-byte swizzle, so a block is a
@@ -42,7 +45,9 @@ namespace {
 
 constexpr int kGroup = 128, kGroups = kWideRows / kGroup;   // rows of one MMA
 constexpr int kStagers = 128;                               // of K, and as many of V
-constexpr int kWideIssuer = kWideRows + 2 * kStagers, kWideThreads = kWideIssuer + 32 * kGroups;
+constexpr int kWideIssuer = kWideRows + 2 * kStagers, kWideCopier = kWideIssuer + 32 * kGroups;
+constexpr int kWideThreads = kWideCopier + 32;
+constexpr int kRing = 4, kAhead = 2;                        // tiles as they lie in the page; on their way
 
 template <int HL>
 struct WideLayout {
@@ -51,13 +56,13 @@ struct WideLayout {
 	static constexpr int kK = 2 * kAttnTile * 64;        // a block's rows of high parts, then low ones
 	static constexpr int kV = HL * 64, kP = kGroup * 64;
 	static constexpr int kOffK = kGroups * NB * kQ, kOffV = kOffK + 2 * NB * kK, kOffP = kOffV + 2 * kV;
-	static constexpr int kOffRaw = kOffP + kGroups * kP;
+	static constexpr int kOffRaw = kOffP + 2 * kGroups * kP;
 	// a tile as it lies in the page; V's rows by fours with 16 bytes between, so that 8
 	// lanes that read 4 rows each find them in banks of their own
 	static constexpr int kCodes = kAttnTile * HL / 2, kScales = kAttnTile * NB * 2;
 	static constexpr int kRawKS = kCodes, kRawV = kCodes + kScales;
 	static constexpr int kRawVS = kRawV + kCodes + kAttnTile / 4 * 16, kRaw = kRawVS + kScales;
-	static constexpr int kBytes = kOffRaw + 2 * kRaw, kSmem = kBytes + 1024;   // to align the base
+	static constexpr int kBytes = kOffRaw + kRing * kRaw, kSmem = kBytes + 1024;   // to align the base
 	// columns: a group's two S (high parts' scores, then low ones') and its O
 	static constexpr int kTmemS = 2 * kAttnTile, kTmemO = 2 * kTmemS, kTmemGroup = 256, kTmem = kGroups * kTmemGroup;
 	static_assert(kRaw % 16 == 0 && kTmemO + HL <= kTmemGroup && kTmem <= 512, "sizes");
@@ -140,9 +145,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b)
 	return d;
 }
 
-// the stagers' own barrier
-__device__ __forceinline__ void bar_stagers() { asm volatile("bar.sync 1, %0;" ::"n"(2 * kStagers) : "memory"); }
-
 // a pair of codes less 8, exact: from low nibbles of bytes 0 and 2 (1024 + c in fp16), from
 // high ones (1024 + 16 c)
 __device__ __forceinline__ __half2 pair_low(uint32_t w)
@@ -173,15 +175,20 @@ __device__ __forceinline__ void words_of(const uint8_t *p, uint32_t (&w)[NW])
 	}
 }
 
+// grid: the plan's items.  A 2048-token prompt (32 heads on 8, 34 GFLOP) takes 128 us, 268
+// TFLOP/s (kvattn.cu's kernel: 193).  A tile of 256 x 32 scores takes 2600 clocks: its
+// products are 700 of the tensor cores', the rest is latency, of which the rows' steps
+// (a wait that finds its barrier done 200 to 300, scores 360, softmax 860, the hand-over
+// of P 330) and the issue of small products one after the other (120 each) are the most.
 template <typename T, int HL>
 __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_constant__ AttnArgs a)
 {
 	using WL = WideLayout<HL>;
 	constexpr int NB = WL::NB;
 	extern __shared__ uint8_t smem_raw[];
-	__shared__ uint64_t bar_s[kGroups][2], p_ready[kGroups], bar_o[kGroups][2], s_free[kGroups][2];
-	__shared__ uint64_t k_ready[2], v_ready[2];
-	__shared__ int have_s[2];   // halves of a tile that are there
+	__shared__ uint64_t bar_s[kGroups][2], p_ready[kGroups][2], bar_o[kGroups][2], s_free[kGroups][2];
+	__shared__ uint64_t k_ready[2], v_ready[2], k_free[2], v_free[2], raw_ready[kRing], raw_free[kRing];
+	__shared__ int have_s[kRing];   // halves of a tile that are there
 	__shared__ uint32_t tmem_at;
 	// what the stagers found in a tile's V scales: factors for the sums so far, keys whose
 	// scale of a block is not finite; and the factors that the sums have by now
@@ -198,22 +205,30 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 	const uint32_t sa = smem_addr(sm);
 	const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 	const int tid = threadIdx.x % 128;   // of a group's rows, or the stagers of K or V
-	const bool row_warp = threadIdx.x < kWideRows, issuer = threadIdx.x >= kWideIssuer;
+	const bool row_warp = threadIdx.x < kWideRows, copier = threadIdx.x >= kWideCopier;
+	const bool issuer = threadIdx.x >= kWideIssuer && !copier;
 	const bool k_stager = !row_warp && threadIdx.x < kWideRows + kStagers;
 
 	griddep_launch_dependents();
 	Item it;
 	if (!cta_item<kWideRows, true>(a, blockIdx.x, it))
 		return;
+	const int groups = (it.rows + kGroup - 1) / kGroup;   // that have rows
 	if (threadIdx.x == 0) {
 		for (int b = 0; b < 2; b++) {
 			mbar_init(&k_ready[b], kStagers / 32);
 			mbar_init(&v_ready[b], kStagers / 32);
+			mbar_init(&k_free[b], groups);
+			mbar_init(&v_free[b], groups);
+		}
+		for (int b = 0; b < kRing; b++) {
+			mbar_init(&raw_ready[b], 1);
+			mbar_init(&raw_free[b], 2 * kStagers / 32);
 		}
 		for (int g = 0; g < kGroups; g++) {
-			mbar_init(&p_ready[g], kGroup / 32);
 			for (int b = 0; b < 2; b++) {
 				mbar_init(&bar_s[g][b], 1);
+				mbar_init(&p_ready[g][b], kGroup / 32);
 				mbar_init(&bar_o[g][b], 1);
 				mbar_init(&s_free[g][b], kGroup / 32);
 			}
@@ -227,7 +242,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 		asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
 	}
 
-	// ---- the key tiles t0, t0 + 1, ..: lane l of every warp of K's stagers keeps the pages of the next
+	// ---- the key tiles t0, t0 + 1, ..: lane l of the copier keeps the pages of the next
 	// 32 of them (two where a page is half a tile)
 	const int ntile = it.t1 - it.t0;
 	const int32_t *table = a.b.table + it.b * a.b.table_stride;
@@ -258,12 +273,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 	};
 	const int half_rec = (HL / 2 + HL / 16) << a.b.page_log2;
 	const uint8_t *head_pages = a.pages + 2 * (int64_t)it.kvh * half_rec;
-	// tile i's bytes on their way to ring stage i % 2: a stager of K has a 16-byte chunk of
-	// the codes of K and of V (head_len 64: of one), some one of the scales
+	// tile i's bytes on their way to its place in the ring, 16 bytes a lane and copy
 	constexpr int CH = WL::kCodes / 16, CR = HL / 32;   // chunks of a tile's codes, of a row's
-	constexpr int SC = WL::kScales / 16, SR = 8 / NB;   // of its scales, rows of one
-	const int my = tid % CH, my_row = my / CR, my_v = tid / CH;
-	const int sc_v = tid / SC, sc_row = tid % SC * SR;
+	constexpr int SC = WL::kScales / 16;                // of its scales
 	auto issue = [&](int i) {
 		if ((i & 31) == 0)
 			load_pages(i);
@@ -271,26 +283,30 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 		const int pa = __shfl_sync(0xffffffffu, page_a, i & 31);
 		const int pb = small ? __shfl_sync(0xffffffffu, page_b, i & 31) : pa;
 		const int have = needs(k0) & ((pa >= 0 ? 1 : 0) | (pb >= 0 ? 2 : 0));
-		const uint32_t st = sa + WL::kOffRaw + (i & 1) * WL::kRaw;
-		// the row's place in its page: 16 rows a page, or this tile's rows of a larger one
-		const int r0 = small ? 0 : k0 & (P - 1), mask = small ? 15 : 31;
-		if (have >> (my_row / 16) & 1) {
-			const uint8_t *src = head_pages + (int64_t)(my_row / 16 ? pb : pa) * a.page_bytes +
-					     ((r0 + (my_row & mask)) * (HL / 2) + my % CR * 16);
-			if (CH == kStagers || my_v == 0)
-				copy16(st + my * 16, src);
-			if (CH == kStagers || my_v == 1)
-				copy16(st + WL::kRawV + my_row / 4 * 16 + my * 16, src + half_rec);
+		const uint32_t st = sa + WL::kOffRaw + i % kRing * WL::kRaw;
+		const int r0 = k0 & (P - 1);
+#pragma unroll
+		for (int h = 0; h < 2; h++) {
+			if (!(have >> h & 1))
+				continue;
+			// the half's first row: in the tile's page, or another page's first
+			const int at = small ? 0 : r0 + 16 * h;
+			const uint8_t *k = head_pages + (int64_t)(h ? pb : pa) * a.page_bytes;
+			const uint8_t *codes = k + at * (HL / 2) + lane * 16;
+			const uint8_t *scales = k + ((HL / 2) << a.b.page_log2) + at * NB * 2;
+#pragma unroll
+			for (int x = 0; x < CH / 64; x++) {
+				const int j = h * (CH / 2) + 32 * x + lane, row = j / CR;
+				copy16(st + j * 16, codes + 512 * x);
+				copy16(st + WL::kRawV + row / 4 * 16 + j * 16, codes + 512 * x + half_rec);
+			}
+			const int isv = lane >= SC / 2, j = lane - isv * (SC / 2);
+			if (lane < SC)
+				copy16(st + (isv ? WL::kRawVS : WL::kRawKS) + (h * (SC / 2) + j) * 16,
+				       scales + isv * half_rec + j * 16);
 		}
-		if (tid < 2 * SC && (have >> (sc_row / 16) & 1))
-			copy16(st + (sc_v ? WL::kRawVS : WL::kRawKS) + tid % SC * 16,
-			       head_pages + (int64_t)(sc_row / 16 ? pb : pa) * a.page_bytes +
-				       (sc_v * half_rec + ((HL / 2) << a.b.page_log2) +
-					(r0 + (sc_row & mask)) * NB * 2));
 		return have;
 	};
-	// groups with rows; the thread's (rows, issuers)
-	const int groups = (it.rows + kGroup - 1) / kGroup;
 	const int group = row_warp ? threadIdx.x / kGroup : issuer ? warp - kWideIssuer / 32 : 0;
 	const int row = group * kGroup + tid;
 	// ---- the row's query: block b's values in the order that the codes come apart in
@@ -371,7 +387,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 		return __any_sync(0xffffffffu, large);
 	};
 	auto stage_k = [&](int i) {
-		const uint8_t *raw = sm + WL::kOffRaw + (i & 1) * WL::kRaw;
+		const uint8_t *raw = sm + WL::kOffRaw + i % kRing * WL::kRaw;
 		const int j = tid / 4, c = tid % 4;   // key row, 16-byte chunk of its slices
 		uint32_t w[NB], d[NB / 2];
 		words_of<NB>(raw + j * (HL / 2) + c * 4 * NB, w);
@@ -408,7 +424,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 		v_top[k] = 0x04000400u;   // 2^-14
 	}
 	auto stage_v = [&](int i, int have) {
-		const uint8_t *raw = sm + WL::kOffRaw + (i & 1) * WL::kRaw;
+		const uint8_t *raw = sm + WL::kOffRaw + i % kRing * WL::kRaw;
 		const int k0 = key0(i);
 		uint32_t bad[NB];   // keys whose scale of a block is not finite
 		bool any_bad = false;
@@ -529,6 +545,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 			mma_slice<2 * kAttnTile>(tg + (i & 1) * WL::kTmemS, sa + (group * NB + b) * WL::kQ,
 						 sa + WL::kOffK + ((i & 1) * NB + b) * WL::kK, b == 0);
 		mma_commit(&bar_s[group][i & 1]);
+		mma_commit(&k_free[i & 1]);
 	};
 
 	fence_proxy_async();   // Q
@@ -541,7 +558,22 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 	float bias = kNoMax, l = 0.0f;   // kLift - the largest score so far, and the weights' sum
 	uint32_t poison = 0;             // blocks of V of which the row has seen a NaN
 	const uint32_t tq = tg + ((uint32_t)(32 * (warp % 4)) << 16);   // the warp's lanes
-	if (issuer) {
+	if (copier) {
+		for (int j = 0; j < ntile + kAhead; j++) {
+			if (j < ntile) {
+				if (j >= kRing)
+					wait(&raw_free[j % kRing], j / kRing - 1);
+				const int have = issue(j);
+				if (lane == 0)
+					have_s[j % kRing] = have;
+			}
+			copies_commit();
+			copies_wait<kAhead>();   // tile j - kAhead is there
+			__syncwarp();
+			if (j >= kAhead && lane == 0)
+				mbar_arrive(&raw_ready[(j - kAhead) % kRing]);
+		}
+	} else if (issuer) {
 		if (lane == 0 && ntile > 0 && group < groups) {
 			wait(&k_ready[0], 0);
 			fence_after();
@@ -557,55 +589,40 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 						issue_s(i + 1);
 				}
 				wait(&v_ready[i & 1], i / 2);
-				wait(&p_ready[group], i);
+				wait(&p_ready[group][i & 1], i / 2);
 				fence_after();
 				if (!failed) {
-					mma_slice<HL>(tg + WL::kTmemO, sa + WL::kOffP + group * WL::kP,
+					mma_slice<HL>(tg + WL::kTmemO, sa + WL::kOffP + (2 * group + (i & 1)) * WL::kP,
 						      sa + WL::kOffV + (i & 1) * WL::kV, i == 0);
 					mma_commit(&bar_o[group][i & 1]);
+					mma_commit(&v_free[i & 1]);
 				}
 			}
 		}
 	} else if (!row_warp) {
-		if (k_stager && ntile > 0) {
-			const int have = issue(0);
-			if (tid == 0)
-				have_s[0] = have;
-		} else if (tid < NB) {
+		if (tid < NB && !k_stager)
 			v_unit[tid] = 1.0f / 32768.0f;
-		}
-		copies_commit();
 #pragma unroll 1
 		for (int j = 0; j < ntile; j++) {
-			copies_wait<0>();
-			bar_stagers();   // tile j is there, and tile j - 1's place free
+			wait(&raw_ready[j % kRing], j / kRing);
+			if (j >= 2)
+				wait(k_stager ? &k_free[j & 1] : &v_free[j & 1], j / 2 - 1);
 			if (k_stager) {
-				if (j + 1 < ntile) {
-					const int have = issue(j + 1);
-					if (tid == 0)
-						have_s[(j + 1) & 1] = have;
-				}
-				copies_commit();
-				if (j >= 2)
-					for (int g = 0; g < groups; g++)
-						wait(&s_free[g][j & 1], j / 2 - 1);
 				stage_k(j);
-				give(&k_ready[j & 1]);
 			} else {
-				const int have = have_s[j & 1];
-				if (j >= 2)
-					for (int g = 0; g < groups; g++)
-						wait(&bar_o[g][j & 1], j / 2 - 1);
+				const int have = have_s[j % kRing];
 				stage_v(j, have);
 				if (tid / 32 == 0) {
-					const bool large = k_is_large(sm + WL::kOffRaw + (j & 1) * WL::kRaw);
+					const bool large = k_is_large(sm + WL::kOffRaw + j % kRing * WL::kRaw);
 					if (tid == 0) {
 						found_s[j & 1].have = have;
 						found_s[j & 1].k_mul = large ? 16.0f : 1.0f;
 					}
 				}
-				give(&v_ready[j & 1]);
 			}
+			give(k_stager ? &k_ready[j & 1] : &v_ready[j & 1]);
+			if (lane == 0)
+				mbar_arrive(&raw_free[j % kRing]);
 		}
 	} else if (group < groups) {
 		// sums so far by a factor of the row's own, and of the blocks'
@@ -672,8 +689,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 			}
 			sum[0] = add2(sum[0], sum[1]);
 			l += sum[0].x + sum[0].y;
-			if (i > 0) {
-				wait(&bar_o[group][(i - 1) & 1], (i - 1) / 2);   // the sums and P's place are free
+			// (P's place is free: S of this tile came after O += P V of tile i - 2)
+			if (i > 0 && (raise || fd.shrinks)) {
+				wait(&bar_o[group][(i - 1) & 1], (i - 1) / 2);
 				fence_after();
 				if (fd.shrinks)   // V's factors of this tile
 					rescale(1.0f, fd.shrink);
@@ -686,9 +704,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 					poison |= seen & fd.bad[b] ? 1u << b : 0u;
 #pragma unroll
 			for (int c = 0; c < 4; c++)
-				*reinterpret_cast<uint4 *>(sm + WL::kOffP + group * WL::kP + slice_at(tid, c)) =
+				*reinterpret_cast<uint4 *>(sm + WL::kOffP + (2 * group + (i & 1)) * WL::kP + slice_at(tid, c)) =
 					make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
-			give(&p_ready[group]);
+			give(&p_ready[group][i & 1]);
 		};
 #pragma unroll 1
 		for (int i = 0; i < ntile; i++) {

@@ -166,10 +166,11 @@ def attention_bounds(dtype, size, vmax, n_rows, out, lse):
     terms), scaled and added over at most 8 blocks (2^-24 each): 2^-20 of sum |q k|.
     A weight: exp of that, of an argument rounded to 2^-23 of its size, and of the
     2-ulp exponential: 2^-20 size + 2^-20; it moves numerator and denominator.
-    Weighted sums: a chain of products 16 rows long each (n / 64 of them or fewer a
-    warp, 2^-23), joined over 4 warps and the runs.  16-bit rows: a weight is
-    rounded to fp16 before and after its row's scale multiplies it (2^-11 each), the
-    result to its type (half of eps)."""
+    Weighted sums: a chain of n / 16 products of 16 rows each, every sum cut to 24
+    bits (2^-24 of sums that grow evenly, half the last on average: n / 64 * 2^-23),
+    joined over the runs.  16-bit rows: a weight is rounded to fp16, and once more
+    with its row's scale or its value is (2^-11 each), the result to its type (half
+    of eps)."""
     e = 2.0 ** -20 * size[..., None] + 2.0 ** -20
     tol = vmax * (2 * e + (n_rows / 64 + 16) * 2.0 ** -23)
     if dtype != torch.float32:

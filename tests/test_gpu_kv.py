@@ -513,6 +513,63 @@ def test_attention_in_place_shared_pages(m, dtype):
     assert torch.equal(same, out) and torch.equal(lse, lse2)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("D,KVH,G,P,q_len,kv_len,causal,window", [
+    (128, 1, 4, 64, [64], [64], True, 0),              # one whole item of 256 query rows
+    (128, 2, 4, 32, [65, 96], [2065, 96], True, 0),    # rows of a second item; several runs
+    (64, 1, 8, 16, [33, 200], [33, 1000], True, 0),    # pages of half a tile
+    (128, 1, 1, 128, [300, 1, 7], [300, 900, 7], True, 0),   # a prompt beside decode steps
+    (64, 2, 5, 256, [27, 130, 2], [50, 600, 2], True, 100),
+    (128, 1, 16, 32, [9, 40], [40, 333], False, 0),
+    (64, 1, 129, 64, [3, 1], [70, 70], True, 0)])      # rows of a token over two items
+def test_attention_many_queries(m, D, KVH, G, P, q_len, kv_len, causal, window, dtype):
+    """sequences of 128 query rows of a KV head and more, alone and beside small ones; K scales
+    over all of fp16's range (above 2^13 and subnormal), V scales that grow from tile to
+    tile; what no query sees may hold anything"""
+    c = Case(m, q_len, kv_len, KVH, D, P, pad=2, seed=sum(kv_len))
+    q = rand(3, c.T, KVH * G, D, dtype=TYPES[dtype], sd=1.2).cuda()
+    out, lse = c.attend(q, causal, window)
+    assert c.cache.status() == 0
+    c.check(q, out, lse, causal, window)
+    # K of a row, V of a tile far apart
+    rng = np.random.default_rng(1)
+    for b, n in enumerate(kv_len):
+        for r in range(n):
+            at = (c.table[b, r // P], slice(None), slice(None), r % P)
+            f = np.array([2.0 ** rng.integers(-16, 17), 2.0 ** min(r // 32 - 9, 9)], np.float32)
+            sc = c.pool.scales()[at].view(np.float16).astype(np.float32)
+            c.pool.scales()[at] = np.clip(sc * f[:, None], -65504, 65504).astype(np.float16).view(np.uint16)
+        c.k[b], c.v[b] = (c.pool.sequence(c.table[b], n, w) for w in (0, 1))
+    c.pages.copy_(torch.tensor(c.pool.data.reshape(-1)))
+    top = max(float(np.abs(k).max()) for k in c.k)
+    out, lse = c.attend(q, causal, window, scale=3.0 / top)
+    assert c.cache.status() == 0
+    c.check(q, out, lse, causal, window, scale=3.0 / top)
+    again, lse2 = c.attend(q, causal, window, scale=3.0 / top)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+def test_attention_many_queries_poisoned(m):
+    """a NaN scale of K or of a block of V reaches the queries that see its row, there its
+    block, and no others"""
+    D, G, kv = 128, 4, 100
+    c = Case(m, [kv], [kv], 1, D, 32, pad=0)
+    q = rand(5, kv, G, D, dtype=torch.bfloat16).cuda()
+    clean, _ = c.attend(q)
+    for which, block, row in ((1, 2, 40), (0, 1, 70)):
+        old = c.pool.data.copy()
+        c.pool.scales()[c.table[0, row // 32], :, which, row % 32, block] = 0x7e00
+        c.pages.copy_(torch.tensor(c.pool.data.reshape(-1)))
+        out, _ = c.attend(q)
+        assert torch.equal(out[:row], clean[:row])
+        part = out[row:, :, 32 * block:32 * block + 32] if which else out[row:]
+        assert part.isnan().all()
+        if which:
+            keep = [e for e in range(D) if e // 32 != block]
+            assert torch.equal(out[row:, :, keep], clean[row:, :, keep])
+        c.pool.data[...] = old
+
+
 def test_attention_extreme_values(m):
     """queries and cache scales far from 1 (the kernel's fp16 operands are brought to
     its range by powers of two), blocks of values of very different size"""
