@@ -549,6 +549,26 @@ def test_attention_many_queries(m, D, KVH, G, P, q_len, kv_len, causal, window, 
     assert torch.equal(out, again) and torch.equal(lse, lse2)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_attention_many_queries_strides_in_place(m, dtype):
+    """query rows at odd offsets, head-major results; results over the queries; a negative scale;
+    nothing seen by the first queries; no log-sum-exp"""
+    D, KVH, G = 64, 2, 4
+    c = Case(m, [70, 200], [130, 150], KVH, D, 16, pad=2)
+    H = KVH * G
+    wide = rand(4, c.T, H * D + 35, dtype=TYPES[dtype]).cuda()
+    q = wide[:, 33:33 + H * D].unflatten(1, (H, D))
+    q[c.start[-1]:] = 5.0
+    plain, lse = c.attend(q.contiguous(), scale=-0.2)
+    c.check(q, plain, lse, scale=-0.2)
+    out = torch.full((H, c.T, D), 5.0, dtype=q.dtype, device="cuda").transpose(0, 1)
+    o, _ = c.attend(q, scale=-0.2, out=out)
+    assert torch.equal(o, plain)
+    o, l2 = c.attend(q, scale=-0.2, out=q, lse=False)
+    assert torch.equal(q, plain) and (l2 == 6.0).all()
+    assert c.cache.status() == 0
+
+
 def test_attention_many_queries_poisoned(m):
     """a NaN scale of K or of a block of V reaches the queries that see its row, there its
     block, and no others"""
