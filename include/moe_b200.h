@@ -499,7 +499,8 @@ MOE_API int moe_kv_gather(moe_kv_cache *cache, const moe_kv_batch *batch, const 
  * once more with V's scale (sequences of 256 and more query rows a KV head round
  * code * scale of V instead, and K scales below 2^-10 beside one above 2^13; fp32
  * rows: q and weights as two fp16 halves, about 22 bits); sums and softmax
- * statistics are fp32.  Rows that a query does not see never reach
+ * statistics are held in fp32 (below 256 query rows, 16-bit rows' products enter
+ * a sum with about 17 bits).  Rows that a query does not see never reach
  * its result, whatever they hold.
  * workspace: 16-byte aligned, at least moe_kv_attention_workspace bytes (which
  * follow from n_heads, the cache and the batch's n_seqs, n_tokens, max_q and

@@ -15,8 +15,8 @@
 // With the cache as the 16-row operand a decode step's few queries (the heads
 // of a KV head's group) fill 8 columns instead of 16 rows, and the codes go
 // from shared memory to operand registers without a transposition: the page
-// layout places a thread's nibbles of all blocks side by side, and a nibble
-// masked out in place is an fp16 subnormal.  S^T comes out with a row per lane
+// layout places a thread's nibbles of all blocks side by side, and a nibble is an
+// fp16 number after one or two operations on a pair.  S^T comes out with a row per lane
 // group and P^T wants a column per lane group: one movmatrix per 8 x 8 tile
 // turns it.
 //
@@ -97,23 +97,33 @@ __device__ __forceinline__ uint32_t smem_addr(const void *p)
 	return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
-// Codes as fp16 subnormals: nibbles masked out in place are code * 2^-24 (low
-// nibbles of bytes 0 and 2) and code * 2^-20 (high ones), exact operands of the
-// products for one logic operation a pair.  The -8 of a code: RAW leaves it to
-// the caller, otherwise one exact fp16 subtraction takes it off.
-template <bool RAW>
+// Codes as fp16 numbers, a pair from a word's low nibbles (bytes 0 and 2) or high ones.
+// 16-bit rows: masked out in place, subnormals code * 2^-24 and code * 2^-20, for one
+// logic operation; the -8 of a code is the caller's (RAW) or one exact subtraction more.
+// The tensor cores line sums up by a subnormal's nominal exponent, so these sums carry
+// about 17 bits, 2^-6 of what rounding the weights costs.  fp32 rows (with subnormals
+// 8.4e-6 off, 4.7e-7 so): code - 8 itself (EXACT), from 1024 + code or 1024 + 16 code; for
+// all rows that takes 134 us instead of 124 for 4 sequences of 131072 rows, without RAW
+// 144.
+template <bool RAW, bool EXACT>
 __device__ __forceinline__ uint32_t codes_low(uint32_t w)
 {
+	static_assert(!(RAW && EXACT), "one or the other");
 	const uint32_t x = w & 0x000f000fu;
+	if (EXACT)
+		return h2_bits(__hsub2(bits_h2(x | 0x64006400u), bits_h2(0x64086408u)));
 	return RAW ? x : h2_bits(__hsub2(bits_h2(x), bits_h2(0x00080008u)));
 }
-template <bool RAW>
+template <bool RAW, bool EXACT>
 __device__ __forceinline__ uint32_t codes_high(uint32_t w)
 {
 	const uint32_t x = w & 0x00f000f0u;
+	if (EXACT)
+		return h2_bits(__hfma2(bits_h2(x | 0x64006400u), bits_h2(0x2c002c00u),   // / 16
+				       bits_h2(0xd480d480u)));                           // - 72
 	return RAW ? x : h2_bits(__hsub2(bits_h2(x), bits_h2(0x00800080u)));
 }
-constexpr float kCodeUnit = 16777216.0f;   // 2^24
+constexpr float kCodeUnit = 16777216.0f;   // 2^24: low nibbles as subnormals
 
 // The tile row that stands as row j of A (of 8): any order will do that K and V, and
 // so S^T and P^T, share.  This one lets the 8 rows that a shared-memory read takes
@@ -174,8 +184,10 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas<HL, NT>) kv_attn_kerne
 	constexpr int RPN = SPLIT ? 4 : 8;            // rows of an 8-column tile
 	constexpr int RPT = RPN * NT, NB = HL / 32;
 	constexpr bool QR = kQInRegs<HL, NT>;
-	// one column tile: the keys' -8 sum to -8 sum q, where the scores' sums start
-	constexpr bool KRAW = NT == 1;
+	// 16-bit rows, one column tile: the keys' -8 sum to -8 sum q, where the scores' sums
+	// start
+	constexpr bool KRAW = NT == 1 && !SPLIT;
+	constexpr float unit = SPLIT ? 1.0f : kCodeUnit, high_unit = SPLIT ? 1.0f : 0.0625f;   // of low nibbles; high ones count 16-fold
 	using SL = StageLayout<HL>;
 	extern __shared__ __align__(128) uint8_t smem[];
 	__shared__ uint2 sm_q[kAttnWarps][QR ? 1 : 2 * NB * NT][32];
@@ -346,7 +358,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas<HL, NT>) kv_attn_kerne
 				x[k] *= __int_as_float((e - 127 + 127) << 23);
 		}
 		// a query with an infinity or a NaN has no finite scores: NaN
-		const float qs = bad ? __int_as_float(0x7fffffff) : scalbnf(a.scale2 * kCodeUnit, -e);
+		const float qs = bad ? __int_as_float(0x7fffffff) : scalbnf(a.scale2 * unit, -e);
 #pragma unroll
 		for (int k = 0; k < HL / 4; k++) {
 			const float v = bad ? 0.0f : x[k] * up;
@@ -370,7 +382,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas<HL, NT>) kv_attn_kerne
 		}
 #pragma unroll
 		for (int h = 0; h < HL / 16; h++) {
-			const float u = h & 1 ? 0.0625f : 1.0f;   // high nibbles count 16-fold
+			const float u = h & 1 ? high_unit : 1.0f;
 			const uint2 f = make_uint2(pack_h2(x[4 * h] * u, x[4 * h + 2] * u),
 						   pack_h2(x[4 * h + 1] * u, x[4 * h + 3] * u));
 			if constexpr (QR)
@@ -450,11 +462,11 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas<HL, NT>) kv_attn_kerne
 			lds_words<NB / 2>(ks + 8 * NB * 2, db);
 #pragma unroll
 			for (int b = 0; b < NB; b++) {
-				const uint32_t lo[4] = {codes_low<KRAW>(ka[b]), codes_low<KRAW>(kb[b]),
-							codes_low<KRAW>(ka[b] >> 8), codes_low<KRAW>(kb[b] >> 8)};
-				const uint32_t hi[4] = {codes_high<KRAW>(ka[b]), codes_high<KRAW>(kb[b]),
-							codes_high<KRAW>(ka[b] >> 8),
-							codes_high<KRAW>(kb[b] >> 8)};
+				const uint32_t lo[4] = {codes_low<KRAW, SPLIT>(ka[b]), codes_low<KRAW, SPLIT>(kb[b]),
+							codes_low<KRAW, SPLIT>(ka[b] >> 8), codes_low<KRAW, SPLIT>(kb[b] >> 8)};
+				const uint32_t hi[4] = {codes_high<KRAW, SPLIT>(ka[b]), codes_high<KRAW, SPLIT>(kb[b]),
+							codes_high<KRAW, SPLIT>(ka[b] >> 8),
+							codes_high<KRAW, SPLIT>(kb[b] >> 8)};
 				const float dka = half_of(da[b / 2], b & 1), dkb = half_of(db[b / 2], b & 1);
 #pragma unroll
 				for (int nt = 0; nt < NT; nt++) {
@@ -582,10 +594,10 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas<HL, NT>) kv_attn_kerne
 			const uint32_t t1 = __byte_perm(v0[b / 2], v1[b / 2], sel1);
 			const uint32_t t2 = __byte_perm(v2[b / 2], v3[b / 2], sel0);
 			const uint32_t t3 = __byte_perm(v2[b / 2], v3[b / 2], sel1);
-			const uint32_t lo[4] = {codes_low<false>(t0), codes_low<false>(t1), codes_low<false>(t2),
-						codes_low<false>(t3)};
-			const uint32_t hi[4] = {codes_high<false>(t0), codes_high<false>(t1),
-						codes_high<false>(t2), codes_high<false>(t3)};
+			const uint32_t lo[4] = {codes_low<false, SPLIT>(t0), codes_low<false, SPLIT>(t1), codes_low<false, SPLIT>(t2),
+						codes_low<false, SPLIT>(t3)};
+			const uint32_t hi[4] = {codes_high<false, SPLIT>(t0), codes_high<false, SPLIT>(t1),
+						codes_high<false, SPLIT>(t2), codes_high<false, SPLIT>(t3)};
 			// the rows' weights of this block
 			const __half2 da = both(bits_h2(wa[b / 2]), b & 1), db = both(bits_h2(wb[b / 2]), b & 1);
 #pragma unroll
@@ -689,7 +701,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas<HL, NT>) kv_attn_kerne
 	float iv[NB];   // sums in true size: the codes' unit, the V scales' factors
 #pragma unroll
 	for (int b = 0; b < NB; b++)
-		iv[b] = kCodeUnit / half_of(v_fac[b / 2], b & 1);
+		iv[b] = unit / half_of(v_fac[b / 2], b & 1);
 #pragma unroll
 	for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -706,7 +718,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas<HL, NT>) kv_attn_kerne
 			const float l = h ? l1[nt] : l0[nt], bias = h ? b1[nt] : b0[nt];
 			auto value = [&](int k, int i) {   // i: the first or second of the two
 				const float v = SPLIT ? o[k][nt][2 * i] + o[k][nt][2 * i + 1] : o[k][nt][2 * i + h];
-				return v * (k & 1 ? iv[k / 2] * 0.0625f : iv[k / 2]);
+				return v * (k & 1 ? iv[k / 2] * high_unit : iv[k / 2]);
 			};
 			if (it.runs > 1) {
 				float *pp = a.part + ((int64_t)item * a.part_rows + r) * OS;

@@ -590,6 +590,22 @@ def test_attention_many_queries_poisoned(m):
         c.pool.data[...] = old
 
 
+@pytest.mark.parametrize("D,KVH,G,P", [(128, 4, 1, 64), (64, 1, 7, 16), (256, 1, 8, 32)])
+def test_attention_fp32_error(m, D, KVH, G, P):
+    """Many keys of equal weight: results are 1 / sqrt(n) of V, and an error of the weighted
+    sums counts sqrt(n)-fold.  Of a weight: 2^-20 of the score's size (as in
+    attention_bounds) with a sign of its own, so it keeps its share; sums cut to 24 bits:
+    2^-22 of V's size a product, less than 2^-19 / sqrt(n) of the whole.  Together below
+    2^-18 = 3.8e-6 of the results' norm; sums of 17 bits would be above 8e-6."""
+    n = 2049
+    c = Case(m, [1], [n], KVH, D, P, pad=0)
+    q = rand(9, 1, KVH * G, D, sd=0.5).cuda()
+    out, _ = c.attend(q)
+    want = ref.attention(f64(q), c.k[0], c.v[0], D ** -0.5)[0]
+    err = np.linalg.norm(f64(out) - want) / np.linalg.norm(want)
+    assert err <= 2.0 ** -18, err
+
+
 def test_attention_extreme_values(m):
     """queries and cache scales far from 1 (the kernel's fp16 operands are brought to
     its range by powers of two), blocks of values of very different size"""
