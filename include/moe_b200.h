@@ -511,7 +511,8 @@ MOE_API int moe_kv_attention(moe_kv_cache *cache, const moe_kv_batch *batch, con
 			     const moe_rows *out, float *lse, float scale, int causal,
 			     int64_t window, void *workspace, size_t workspace_bytes, void *stream);
 /* Waits for the device; MOE_OK, or (once) MOE_ERR_INVALID if a call since the
- * last one met arrays, pages or positions out of range. */
+ * last one met arrays, pages or positions out of range, or MOE_ERR_TIMEOUT if a
+ * bounded wait inside the attention kernel expired. */
 MOE_API int moe_kv_status(moe_kv_cache *cache);
 
 /* ------------------------------------------------------------------ */
