@@ -235,6 +235,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 		}
 		fence_mbar_init();
 	}
+	if (threadIdx.x < NB)   // (rows of an item without tiles wait for nothing but the barrier below)
+		v_unit[threadIdx.x] = 1.0f / 32768.0f;
 	if (warp == 0) {
 		asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
 				     smem_addr(&tmem_at)),
@@ -600,8 +602,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 			}
 		}
 	} else if (!row_warp) {
-		if (tid < NB && !k_stager)
-			v_unit[tid] = 1.0f / 32768.0f;
 #pragma unroll 1
 		for (int j = 0; j < ntile; j++) {
 			wait(&raw_ready[j % kRing], j / kRing);

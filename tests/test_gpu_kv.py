@@ -590,6 +590,22 @@ def test_attention_many_queries_poisoned(m):
         c.pool.data[...] = old
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("q_len,kv_len,causal", [
+    ([64], [0], True), ([64], [0], False), ([200], [100], True),   # queries before the first row
+    ([300, 3, 64, 128], [70, 40, 0, 128], True), ([300], [1], True)])
+def test_attention_many_queries_nothing_seen(m, q_len, kv_len, causal, D, dtype):
+    """items of 256 query rows without a key tile: zeros and -infinity, alone and beside
+    sequences that see rows"""
+    c = Case(m, q_len, kv_len, 2, D, 32, pad=1, seed=1)
+    q = rand(2, c.T, 8, D, dtype=TYPES[dtype]).cuda()
+    for _ in range(3):
+        out, lse = c.attend(q, causal)
+        assert c.cache.status() == 0
+        c.check(q, out, lse, causal)
+
+
 @pytest.mark.parametrize("D,KVH,G,P", [(128, 4, 1, 64), (64, 1, 7, 16), (256, 1, 8, 32)])
 def test_attention_fp32_error(m, D, KVH, G, P):
     """Many keys of equal weight: results are 1 / sqrt(n) of V, and an error of the weighted
