@@ -1,0 +1,104 @@
+"""Attention over the 4-bit cache where an item has many key tiles (rings that turn, pages
+fetched again every 32 tiles, runs at their longest), and the weighted sums over long
+rows against 64 bits by their norm."""
+import numpy as np
+import pytest
+import torch
+
+import kv_ref as ref
+from kv_ref import TYPES, rows
+from test_gpu_kv import LEGACY, Case, cuda_i32, f64, m, rand  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def check_tokens(c, q, out, lse, tokens, window=0, scale=None):
+    """rows of some tokens of a causal call against 64 bits (token by token: its keys cut
+    behind it)"""
+    x, o, l = f64(q), f64(out), f64(lse)
+    scale = scale or c.D ** -0.5
+    for t in tokens:
+        b = int(np.searchsorted(c.start, t, side="right")) - 1
+        n = c.kv_len[b] - (c.start[b + 1] - t) + 1
+        k, v = c.k[b][:n], c.v[b][:n]
+        want, wl, size = ref.attention(x[t:t + 1], k, v, scale, True, window)
+        tol, tol_l = ref.attention_bounds(q.dtype, size, np.abs(v).max(), n, want, wl)
+        err = np.abs(o[t:t + 1] - want)
+        assert (err <= tol).all(), f"token {t}: {(err / tol).max():.3g} of its bound"
+        assert (np.abs(l[t:t + 1] - wl) <= tol_l).all(), f"token {t}: lse"
+
+
+def some(rng, start, n=10):
+    """the first and last tokens and some between"""
+    end = int(start[-1])
+    return sorted({0, 1, end - 1, *(int(x) - 1 for x in start[1:]), *(int(x) for x in rng.integers(0, end, n))})
+
+
+@pytest.mark.parametrize("dtype,D,KVH,G,P,q_len,kv_len,window", [
+    ("bf16", 128, 8, 4, 64, [512], [2048], 0),      # items of 256 query rows, runs of some 50 tiles
+    ("f16", 64, 8, 4, 16, [512], [2077], 0),        # the same from pages of half a tile
+    ("bf16", 128, 8, 4, 32, [300, 512], [300, 2500], 1500),
+    ("f32", 128, 8, 8, 128, [600], [2100], 0),      # an item a warp: whole sequences of 66 tiles
+    ("f32", 256, 4, 8, 16, [600], [2100], 0),
+    ("bf16", 256, 4, 16, 64, [600], [2100], 1700)])
+def test_attention_long_items(m, dtype, D, KVH, G, P, q_len, kv_len, window):
+    """prompts over long rows: every buffer of a kernel's rings comes round many times, the
+    pages' list is fetched anew, V's scales grow on the way (sums are rescaled)"""
+    c = Case(m, q_len, kv_len, KVH, D, P, pad=1, seed=D + P)
+    q = rand(11, c.T, KVH * G, D, dtype=TYPES[dtype], sd=1.2).cuda()
+    tokens = some(np.random.default_rng(P), c.start)
+    out, lse = c.attend(q, window=window)
+    assert c.cache.status() == 0
+    check_tokens(c, q, out, lse, tokens, window)
+    for b, n in enumerate(kv_len):
+        at = np.arange(n)
+        f = np.float32(2.0) ** np.minimum(at // 150 - 9, 5)
+        pages, row = c.table[b, at // P], at % P
+        sc = c.pool.scales()[pages, :, 1, row].view(np.float16).astype(np.float32)
+        c.pool.scales()[pages, :, 1, row] = (sc * f[:, None, None]).astype(np.float16).view(np.uint16)
+        c.v[b] = c.pool.sequence(c.table[b], n, 1)
+    c.pages.copy_(torch.tensor(c.pool.data.reshape(-1)))
+    out, lse = c.attend(q, window=window)
+    assert c.cache.status() == 0
+    check_tokens(c, q, out, lse, tokens, window)
+    again, lse2 = c.attend(q, window=window)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("dtype,D,G", [("f32", 64, 2), ("bf16", 64, 4), ("f16", 128, 4), ("bf16", 256, 3)])
+def test_attention_long_decode_items(m, dtype, D, G):
+    """decode steps of 128 sequences that share their pages, in runs of more than 32 tiles"""
+    KVH, P, n = 8, 32, 2100
+    c = Case(m, [1], [n], KVH, D, P, seed=G)
+    B = 128
+    lens = [n - 7 * b for b in range(B)]
+    c.q_len, c.kv_len, c.k, c.v = [1] * B, lens, c.k * B, c.v * B
+    c.k, c.v = ([x[:i] for x, i in zip(y, lens)] for y in (c.k, c.v))
+    c.table = np.repeat(c.table, B, 0)
+    c.start, c.T = np.arange(B + 1, dtype=np.int32), B
+    c.dev = [torch.tensor(x, device="cuda") for x in (c.start, np.array(lens, np.int32), c.table)]
+    c.batch = m.KVBatch(B, B, 1, n, *[x.data_ptr() for x in c.dev], c.table.shape[1])
+    q = rand(12, B, KVH * G, D, dtype=TYPES[dtype], sd=1.2).cuda()
+    out, lse = c.attend(q)
+    assert c.cache.status() == 0
+    check_tokens(c, q, out, lse, range(0, B, 9))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("D,KVH,G,P,n", [(128, 4, 1, 64, 1), (64, 1, 7, 16, 1), (256, 1, 8, 32, 1), (128, 2, 4, 64, 64),
+                                         (64, 1, 8, 32, 33)])
+def test_attention_error_of_many_rows(m, dtype, D, KVH, G, P, n):
+    """Many keys of equal weight: results are 1 / sqrt(rows) of V.  A weight and its product with
+    V's scale (or the weight, and V's value) are rounded to fp16, 2^-11 of their size each with
+    signs of their own, so the sums keep the share: sqrt(2) 2^-11 of the results' norm.  Codes
+    as subnormals, 2^-16 of a product a sum of 16 rows at most, all of one sign: sqrt(rows) / 16
+    * 2^-16 = 2^-14.5 for 2049.  The results' rounding: half of eps.  Scores: 2^-19 of the
+    weights.  The rest is below 2^-18."""
+    c = Case(m, [n], [2049], KVH, D, P, pad=0)
+    q = rand(9, n, KVH * G, D, sd=0.5, dtype=TYPES[dtype]).cuda()
+    out, _ = c.attend(q, causal=False)
+    k, v = (torch.tensor(x[0], dtype=torch.float64, device="cuda").repeat_interleave(G, 1) for x in (c.k, c.v))
+    p = torch.einsum("thd,shd->hts", q.double(), k).mul_(D ** -0.5).softmax(-1)
+    want = torch.einsum("hts,shd->thd", p, v)
+    err = ((out.double() - want).norm() / want.norm()).item()
+    assert err <= 2.0 ** -10.5 + 2.0 ** -14.5 + 2.0 ** -17 + torch.finfo(q.dtype).eps / 2, err
