@@ -10,8 +10,8 @@
 // number exactly, down to the smallest scale: two rows of B a key, whose scores the rows
 // add.  (Codes alone, with a sum a block and its scale in fp32, cost the rows four times
 // the tensor memory reads and a shared-memory read of 128 scales a tile: 148 us for a
-// 2048-token prompt.)  Above 2^13 a product may not fit: tiles with such a scale take
-// theirs times 2^-4.
+// 2048-token prompt.)  From 2^13 on a product may not fit (-8 * 2^13 is above 65504): keys
+// with such a scale take theirs times 2^-4, and their scores 2^4.
 // V's scales are rounded in: a weight and a value are rounded to fp16 once each, as often
 // as kvattn.cu rounds (weight, then weight * scale).  They are brought below 2 by a power
 // of two a block, the largest so far to [1, 2).
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 	const int all_hi = a.causal ? min(it.kv, first_row + 1) : it.kv;
 
 	// ---- codes to operands
-	// whether a tile has a K scale above 2^13 (in any row: what no query sees may be scaled
+	// whether a tile has a K scale of 2^13 or more (in any row: what no query sees may be scaled
 	// as well)
 	auto k_is_large = [&](const uint8_t *raw) -> bool {
 		uint32_t d[NB / 2];
@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 		bool large = false;
 #pragma unroll
 		for (int k = 0; k < NB / 2; k++)
-			large |= !__hble2(__habs2(bits_h2(d[k])), bits_h2(0x70007000u));
+			large |= !__hble2(__habs2(bits_h2(d[k])), bits_h2(0x6fff6fffu));
 		return __any_sync(0xffffffffu, large);
 	};
 	auto stage_k = [&](int i) {

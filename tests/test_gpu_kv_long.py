@@ -102,3 +102,23 @@ def test_attention_error_of_many_rows(m, dtype, D, KVH, G, P, n):
     want = torch.einsum("hts,shd->thd", p, v)
     err = ((out.double() - want).norm() / want.norm()).item()
     assert err <= 2.0 ** -10.5 + 2.0 ** -14.5 + 2.0 ** -17 + torch.finfo(q.dtype).eps / 2, err
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("top", [65536.0, -65536.0, 65504.0, 70000.0, 524032.0, 1e9])
+def test_attention_large_keys(m, top, dtype):
+    """keys whose scale is 2^13 and more, with the code that stands for -8 of it"""
+    D, KVH, G, n = 128, 1, 4, 70
+    c = Case(m, [n], [n], KVH, D, 32, pad=0)
+    x = np.random.default_rng(4).standard_normal((n, KVH, D)).astype(np.float32) * (abs(top) / 8)
+    x = np.clip(x, -abs(top), abs(top))
+    x[::3, :, ::32] = top
+    for r in range(n):
+        c.pool.put(c.table[0, r // 32], r % 32, 0, x[r])
+    c.k[0] = c.pool.sequence(c.table[0], n, 0)
+    c.pages.copy_(torch.tensor(c.pool.data.reshape(-1)))
+    q = rand(5, n, KVH * G, D, dtype=TYPES[dtype]).cuda()
+    scale = 2.0 / min(abs(top), 524032.0)
+    out, lse = c.attend(q, scale=scale)
+    assert c.cache.status() == 0
+    c.check(q, out, lse, scale=scale)
