@@ -497,8 +497,8 @@ MOE_API int moe_kv_gather(moe_kv_cache *cache, const moe_kv_batch *batch, const 
  * strides) and must not overlap it otherwise.  Products take the codes exactly, q
  * in fp16 after a power of two a row, and the weights in fp16, rounded once and
  * once more with V's scale (sequences of 256 and more query rows a KV head round
- * code * scale of V instead, and K scales below 2^-10 beside one above 2^13; fp32
- * rows: q and weights as two fp16 halves, about 22 bits); sums and softmax
+ * code * scale of V instead, and K scales below 2^-10 of a cache row that has one of
+ * 2^13 or more; fp32 rows: q and weights as two fp16 halves, about 22 bits); sums and softmax
  * statistics are held in fp32 (below 256 query rows, 16-bit rows' products enter
  * a sum with about 17 bits).  Rows that a query does not see never reach
  * its result, whatever they hold.

@@ -193,9 +193,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 	// what the stagers found in a tile's V scales: factors for the sums so far, keys whose
 	// scale of a block is not finite; and the factors that the sums have by now
 	struct Found {
-		int have;   // halves of the tile that are there
+		int have;         // halves of the tile that are there; 4: of its keys some are large
+		uint32_t large;   // those whose K is held times 2^-4
 		uint32_t shrinks, bads;
-		float k_mul;   // what the tile's K is to be multiplied with
 		float shrink[NB];
 		uint32_t bad[NB];
 	};
@@ -377,16 +377,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 	const int all_hi = a.causal ? min(it.kv, first_row + 1) : it.kv;
 
 	// ---- codes to operands
-	// whether a tile has a K scale of 2^13 or more (in any row: what no query sees may be scaled
-	// as well)
-	auto k_is_large = [&](const uint8_t *raw) -> bool {
-		uint32_t d[NB / 2];
-		words_of<NB / 2>(raw + WL::kRawKS + lane * NB * 2, d);
+	// whether a key's scales have one of 2^13 or more: a matter of its own row, so what the
+	// others hold (behind the sequence's end, or behind a query) counts for nothing
+	auto k_is_large = [&](const uint32_t (&d)[NB / 2]) -> bool {
 		bool large = false;
 #pragma unroll
 		for (int k = 0; k < NB / 2; k++)
 			large |= !__hble2(__habs2(bits_h2(d[k])), bits_h2(0x6fff6fffu));
-		return __any_sync(0xffffffffu, large);
+		return large;
 	};
 	auto stage_k = [&](int i) {
 		const uint8_t *raw = sm + WL::kOffRaw + i % kRing * WL::kRaw;
@@ -394,7 +392,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 		uint32_t w[NB], d[NB / 2];
 		words_of<NB>(raw + j * (HL / 2) + c * 4 * NB, w);
 		words_of<NB / 2>(raw + WL::kRawKS + j * NB * 2, d);
-		if (k_is_large(raw))
+		if (k_is_large(d))
 #pragma unroll
 			for (int k = 0; k < NB / 2; k++)
 				d[k] = h2_bits(__hmul2(bits_h2(d[k]), bits_h2(0x2c002c00u)));   // 2^-4
@@ -613,10 +611,12 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 				const int have = have_s[j % kRing];
 				stage_v(j, have);
 				if (tid / 32 == 0) {
-					const bool large = k_is_large(sm + WL::kOffRaw + j % kRing * WL::kRaw);
+					uint32_t d[NB / 2];
+					words_of<NB / 2>(sm + WL::kOffRaw + j % kRing * WL::kRaw + WL::kRawKS + lane * NB * 2, d);
+					const uint32_t large = __ballot_sync(0xffffffffu, k_is_large(d));
 					if (tid == 0) {
-						found_s[j & 1].have = have;
-						found_s[j & 1].k_mul = large ? 16.0f : 1.0f;
+						found_s[j & 1].have = have | (large ? 4 : 0);
+						found_s[j & 1].large = large;
 					}
 				}
 			}
@@ -645,13 +645,12 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 		auto tile = [&](auto full_c, const float2 (&s)[kAttnTile / 2], int i, uint32_t seen) {
 			constexpr bool FULL = decltype(full_c)::value;   // every row sees all of it
 			const Found &fd = found_s[i & 1];
-			const float qm = qs * fd.k_mul;
 			// ---- weights, times 2^kLift over the largest so far
 			float2 t[kAttnTile / 2];
 			auto weigh = [&]() {
 #pragma unroll
 				for (int j = 0; j < kAttnTile / 2; j++) {
-					t[j] = fma2(s[j], make_float2(qm, qm), make_float2(bias, bias));
+					t[j] = fma2(s[j], make_float2(qs, qs), make_float2(bias, bias));
 					if (!FULL) {
 						t[j].x = seen >> (2 * j) & 1 ? t[j].x : none;
 						t[j].y = seen >> (2 * j + 1) & 1 ? t[j].y : none;
@@ -670,8 +669,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 				float top = none;
 #pragma unroll
 				for (int j = 0; j < kAttnTile / 2; j++) {
-					top = fmaxf(top, FULL || (seen >> (2 * j) & 1) ? s[j].x * qm : none);
-					top = fmaxf(top, FULL || (seen >> (2 * j + 1) & 1) ? s[j].y * qm : none);
+					top = fmaxf(top, FULL || (seen >> (2 * j) & 1) ? s[j].x * qs : none);
+					top = fmaxf(top, FULL || (seen >> (2 * j + 1) & 1) ? s[j].y * qs : none);
 				}
 				const float next = fminf(bias, kLift - top);
 				f = ex2(next - bias);
@@ -733,6 +732,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 			if (have == 3 && k0 >= all_lo && k0 + kAttnTile <= all_hi) {
 				tile(std::true_type{}, s, i, 0xffffffffu);
 			} else {
+				const uint32_t large = have & 4 ? found_s[i & 1].large : 0;
+				if (large)
+#pragma unroll
+					for (int j = 0; j < kAttnTile / 2; j++) {
+						s[j].x *= large >> (2 * j) & 1 ? 16.0f : 1.0f;
+						s[j].y *= large >> (2 * j + 1) & 1 ? 16.0f : 1.0f;
+					}
 				const int from = min(max(see_lo - k0, 0), 32), to = min(max(see_hi - k0, 0), 32);
 				const uint32_t range = to > from ? 0xffffffffu >> (32 - (to - from)) << from : 0u;
 				tile(std::false_type{}, s, i,

@@ -122,3 +122,41 @@ def test_attention_large_keys(m, top, dtype):
     out, lse = c.attend(q, scale=scale)
     assert c.cache.status() == 0
     c.check(q, out, lse, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("D,P", [(128, 32), (64, 16), (128, 128)])
+def test_attention_small_key_scales(m, D, P, dtype):
+    """Key scales of 2^-14 .. 2^-11 in prompts.  What a row that a query does not see holds
+    (behind the sequence's end; or behind the query, where others see it) changes no bit of its
+    result: zeros, NaN, fp16's largest scale."""
+    KVH, G, n, kv = 2, 4, 83, 83
+    c = Case(m, [n], [kv], KVH, D, P, pad=0, extra=0, spare=0)
+    rng = np.random.default_rng(4)
+    x = rng.standard_normal((kv, KVH, D)).astype(np.float32) * 2.0 ** -11
+    x *= 2.0 ** rng.integers(-1, 2, (kv, KVH, 1))
+    for r in range(kv):
+        c.pool.put(c.table[0, r // P], r % P, 0, x[r])
+    c.k[0] = c.pool.sequence(c.table[0], kv, 0)
+    q = rand(5, n, KVH * G, D, dtype=TYPES[dtype]).cuda()
+    scale = D ** -0.5 * 2.0 ** 11
+    clean = c.pool.data.copy()
+    got = []
+    for bits in (0, 0x7fff, 0x7bff, 0x7c00):
+        c.pool.data[...] = clean
+        for r in range(kv, -(-kv // P) * P):
+            c.pool.scales()[c.table[0, r // P], :, :, r % P] = bits
+        c.pages.copy_(torch.tensor(c.pool.data.reshape(-1)))
+        out, lse = c.attend(q, scale=scale)
+        assert c.cache.status() == 0
+        c.check(q, out, lse, scale=scale)
+        got.append((out, lse))
+    for out, lse in got[1:]:
+        assert torch.equal(out, got[0][0]) and torch.equal(lse, got[0][1])
+    for bits in (0x7fff, 0x7bff, 0x7000):
+        c.pool.data[...] = clean
+        c.pool.scales()[c.table[0, 70 // P], :, 0, 70 % P] = bits
+        c.pages.copy_(torch.tensor(c.pool.data.reshape(-1)))
+        out, lse = c.attend(q, scale=scale)
+        assert torch.equal(out[:70], got[0][0][:70]) and torch.equal(lse[:70], got[0][1][:70])
+        assert c.cache.status() == 0
