@@ -119,6 +119,12 @@ __device__ __forceinline__ bool find_item(const AttnArgs &a, int index, Item &f)
 				all += (float)((n * a.G + RPT - 1) / RPT) * (float)seq_tiles(a, n, kv);
 		run = (int)fminf(ceilf(warp_sum(all) * a.KVH / a.target), (float)kRunMax);
 		run = max(run, kRunMin);
+	} else if (blockIdx.x == 0 && threadIdx.x < 32) {
+		// the walk below ends at the item: here every sequence is looked at, and those
+		// out of range reported
+		for (int b = lane; b < B; b += 32)
+			seq_of(a, b, s0, n, kv);
+		n = 0;
 	}
 	int item0 = 0, tile0 = 0;
 	for (int b0 = 0; b0 < B; b0 += 32) {

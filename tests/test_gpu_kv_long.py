@@ -160,3 +160,24 @@ def test_attention_small_key_scales(m, D, P, dtype):
         out, lse = c.attend(q, scale=scale)
         assert torch.equal(out[:70], got[0][0][:70]) and torch.equal(lse[:70], got[0][1][:70])
         assert c.cache.status() == 0
+
+
+@pytest.mark.parametrize("dtype,q_len,kv,B", [("f32", 1, 20, 100), ("bf16", 2, 32, 70), ("f16", 64, 32, 40)])
+def test_attention_reports_every_sequence(m, dtype, q_len, kv, B):
+    """lengths out of range in a sequence behind the first 32, of a call whose items are whole
+    sequences: reported, and the others are right"""
+    D, KVH, G = 64, 1, 4
+    c = Case(m, [q_len] * B, [kv] * B, KVH, D, 16, pad=2)
+    q = rand(5, c.T, G, D, dtype=TYPES[dtype]).cuda()
+    for b, bad in ((B - 1, kv + 1), (33, -1)):
+        c.dev[1].fill_(kv)
+        c.dev[1][b] = bad
+        out, lse = c.attend(q)
+        assert c.cache.status() == -1 and c.cache.status() == 0
+        c.check(q, out, lse, seqs=[0, 1, 31, 32, B - 2])
+        a, z = c.start[b], c.start[b + 1]
+        assert (out[a:z] == 5.0).all() and (lse[a:z] == 6.0).all()
+    c.dev[1].fill_(kv)
+    c.dev[0][B - 1] -= 1   # a query more for the last sequence than max_q
+    c.attend(q)
+    assert c.cache.status() == -1 and c.cache.status() == 0
