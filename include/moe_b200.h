@@ -497,11 +497,13 @@ MOE_API int moe_kv_gather(moe_kv_cache *cache, const moe_kv_batch *batch, const 
  * strides) and must not overlap it otherwise.  Products take the codes exactly, q
  * in fp16 after a power of two a row, and the weights in fp16, rounded once and
  * once more with V's scale (sequences of 256 and more query rows a KV head round
- * code * scale of V instead, and K scales below 2^-10 of a cache row that has one of
- * 2^13 or more; fp32 rows: q and weights as two fp16 halves, about 22 bits); sums and softmax
- * statistics are held in fp32 (below 256 query rows, 16-bit rows' products enter
- * a sum with about 17 bits).  Rows that a query does not see never reach
- * its result, whatever they hold.
+ * code * scale of V instead, and K scales below 2^-10 of a cache row that has one
+ * of 2^13 or more; fp32 rows: q and weights as two fp16 halves, about 22 bits);
+ * sums and softmax statistics are held in fp32 (below 256 query rows, 16-bit
+ * rows' products enter a sum with about 17 bits; the tensor cores' sums are of 256
+ * products of 16 rows at most, which stay within 2^-15 where all values have one
+ * sign, and are added up in fp32).  Rows that a query does not see never reach its
+ * result, whatever they hold.
  * workspace: 16-byte aligned, at least moe_kv_attention_workspace bytes (which
  * follow from n_heads, the cache and the batch's n_seqs, n_tokens, max_q and
  * max_kv; 0: none needed); what it holds counts for this call only. */

@@ -177,7 +177,7 @@ constexpr int kAttnCtas = HL == 128 && NT == 1 ? 4 : 1;
 // 32 heads on 8: 526 MB in 124 us, 4.25 TB/s of 6.5) are bound by the instructions
 // that take codes apart, a batch of 64 such sequences of up to 4096 rows (72 MB in
 // 37 us) by latency: a few tiles a warp between its plan and its last store.
-template <typename T, int HL, int NT>
+template <typename T, int HL, int NT, bool FOLD>
 __global__ void __launch_bounds__(kAttnThreads, kAttnCtas<HL, NT>) kv_attn_kernel(AttnArgs a)
 {
 	constexpr bool SPLIT = sizeof(T) == 4;        // two columns a row
@@ -633,7 +633,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas<HL, NT>) kv_attn_kerne
 	const int all_lo = a.window ? max(it.lo, last_row - a.window + 1) : it.lo;
 	const int all_hi = a.causal ? min(it.kv, first_row + 1) : it.kv;
 	int stage = 0;
-	for (int i = 0; i < ntile; i++) {
+	auto tile_at = [&](int i) {
 		copies_wait<kAttnStages - 2>();
 		__syncwarp();   // every lane's copies are in, and the stage before is read
 		{
@@ -692,52 +692,91 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas<HL, NT>) kv_attn_kerne
 					rows16(std::false_type{}, st, 16 * u, k0);
 		}
 		stage = stage + 1 == kAttnStages ? 0 : stage + 1;
-	}
-	copies_wait<0>();
+	};
 
 	// ---- out of the registers: a lane has values 2 g, 2 g + 1 of every half block
-	// of its columns' rows, 8 lanes 16 values side by side
+	// of its columns' rows, 8 lanes 16 values side by side.  To the item's record, on top of
+	// what is there (!first), or (last, no other runs) to the results
 	constexpr int OS = HL + 4;
-	float iv[NB];   // sums in true size: the codes' unit, the V scales' factors
+	auto leave = [&](bool first, bool last) {
+		float iv[NB];   // sums in true size: the codes' unit, the V scales' factors
 #pragma unroll
-	for (int b = 0; b < NB; b++)
-		iv[b] = unit / half_of(v_fac[b / 2], b & 1);
+		for (int b = 0; b < NB; b++)
+			iv[b] = unit / half_of(v_fac[b / 2], b & 1);
 #pragma unroll
-	for (int nt = 0; nt < NT; nt++) {
+		for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-		for (int x = 4; x < 32; x *= 2) {
-			l0[nt] += __shfl_xor_sync(0xffffffffu, l0[nt], x);
-			if (!SPLIT)
-				l1[nt] += __shfl_xor_sync(0xffffffffu, l1[nt], x);
-		}
+			for (int x = 4; x < 32; x *= 2) {
+				l0[nt] += __shfl_xor_sync(0xffffffffu, l0[nt], x);
+				if (!SPLIT)
+					l1[nt] += __shfl_xor_sync(0xffffffffu, l1[nt], x);
+			}
 #pragma unroll
-		for (int h = 0; h < (SPLIT ? 1 : 2); h++) {   // the columns' rows: one, or two
-			const int r = nt * RPN + (SPLIT ? c : 2 * c + h);
-			if (r >= it.rows)
-				continue;
-			const float l = h ? l1[nt] : l0[nt], bias = h ? b1[nt] : b0[nt];
-			auto value = [&](int k, int i) {   // i: the first or second of the two
-				const float v = SPLIT ? o[k][nt][2 * i] + o[k][nt][2 * i + 1] : o[k][nt][2 * i + h];
-				return v * (k & 1 ? iv[k / 2] * high_unit : iv[k / 2]);
-			};
-			if (it.runs > 1) {
+			for (int h = 0; h < (SPLIT ? 1 : 2); h++) {   // the columns' rows: one, or two
+				const int r = nt * RPN + (SPLIT ? c : 2 * c + h);
+				const float bias = h ? b1[nt] : b0[nt];
+				float l = h ? l1[nt] : l0[nt], f = 0.0f;
 				float *pp = a.part + ((int64_t)item * a.part_rows + r) * OS;
+				if (!first) {
+					if (r < it.rows) {
+						f = ex2(bias - pp[HL]);   // (the maximum only rises)
+						l = fmaf(pp[HL + 1], f, l);
+					}
+					__syncwarp();   // read by all before one writes it
+				}
+				if (r >= it.rows)
+					continue;
+				auto value = [&](int k, int i) {   // i: the first or second of the two
+					const float v = SPLIT ? o[k][nt][2 * i] + o[k][nt][2 * i + 1] : o[k][nt][2 * i + h];
+					return v * (k & 1 ? iv[k / 2] * high_unit : iv[k / 2]);
+				};
+				auto two = [&](int k) {
+					float2 v = make_float2(value(k, 0), value(k, 1));
+					if (!first) {
+						const float2 w = *reinterpret_cast<const float2 *>(pp + 16 * k + 2 * g);
+						v = make_float2(fmaf(w.x, f, v.x), fmaf(w.y, f, v.y));
+					}
+					return v;
+				};
+				if (!last || it.runs > 1) {
 #pragma unroll
-				for (int k = 0; k < 2 * NB; k++)
-					*reinterpret_cast<float2 *>(pp + 16 * k + 2 * g) =
-						make_float2(value(k, 0), value(k, 1));
-				if (g == 0)
-					*reinterpret_cast<float2 *>(pp + HL) = make_float2(bias, l);
-			} else {
-				const RowOut<T> out(a, it, r, bias, l);
+					for (int k = 0; k < 2 * NB; k++)
+						*reinterpret_cast<float2 *>(pp + 16 * k + 2 * g) = two(k);
+					if (g == 0)
+						*reinterpret_cast<float2 *>(pp + HL) = make_float2(bias, l);
+				} else {
+					const RowOut<T> out(a, it, r, bias, l);
 #pragma unroll
-				for (int k = 0; k < 2 * NB; k++)
-					out.two(16 * k + 2 * g, value(k, 0), value(k, 1));
-				if (g == 0)
-					out.lse();
+					for (int k = 0; k < 2 * NB; k++) {
+						const float2 v = two(k);
+						out.two(16 * k + 2 * g, v.x, v.y);
+					}
+					if (g == 0)
+						out.lse();
+				}
 			}
 		}
+	};
+	for (int i0 = 0;;) {
+		const int i1 = FOLD ? min(i0 + kFold, ntile) : ntile;
+		for (int i = i0; i < i1; i++)
+			tile_at(i);
+		leave(!FOLD || i0 == 0, !FOLD || i1 == ntile);
+		if (!FOLD || i1 == ntile)
+			break;
+		i0 = i1;
+#pragma unroll
+		for (int nt = 0; nt < NT; nt++) {
+			l0[nt] = l1[nt] = 0.0f;
+#pragma unroll
+			for (int k = 0; k < 2 * NB; k++)
+#pragma unroll
+				for (int x = 0; x < 4; x++)
+					o[k][nt][x] = 0.0f;
+		}
+		__syncwarp();   // the record, before it is read
 	}
+	copies_wait<0>();
 }
 
 // ---------------------------------------------------------------- launches
@@ -761,14 +800,16 @@ void plan_items(Plan &p, const moe_kv_cache *c, const moe_kv_batch *b, int64_t G
 	// split unless there are tiles enough, or every sequence is a single run
 	const int64_t longest = (b->max_kv + kAttnTile - 1) / kAttnTile;
 	p.split = p.tiles < 4 * wave && longest > kRunMin;
+	p.folds = (p.split ? p.tiles * longest / p.target + 1 : longest) > kFold;
 	p.items = p.tiles;
 	if (p.split) {
 		const int64_t capped = p.tiles * longest / kRunMax + 1;
 		const int64_t most = p.tiles * ((longest + kRunMin - 1) / kRunMin);
 		p.items += 1 + (capped > p.target ? capped : p.target);
 		p.items = p.items < most ? p.items : most;
-		p.part_bytes = (size_t)(p.items * p.rows * (c->d.head_len + 4) * 4);
 	}
+	if (p.split || p.folds)
+		p.part_bytes = (size_t)(p.items * p.rows * (c->d.head_len + 4) * 4);
 }
 
 // The kernels of a call: an item a warp (`narrow`), an item a CTA (`wide`), or both, each
@@ -812,10 +853,10 @@ cudaError_t launch_attn_as(const AttnArgs &a, const Plan &p, cudaStream_t st)
 {
 	constexpr int RPT = (sizeof(T) == 4 ? 4 : 8) * NT;
 	constexpr int smem = kAttnSmem<HL>;
-	if (cudaError_t e = ensure_smem(kv_attn_kernel<T, HL, NT>, smem))
+	auto kernel = p.folds ? kv_attn_kernel<T, HL, NT, true> : kv_attn_kernel<T, HL, NT, false>;
+	if (cudaError_t e = ensure_smem(kernel, smem))
 		return e;
-	kv_attn_kernel<T, HL, NT>
-		<<<(unsigned)((p.items + kAttnWarps - 1) / kAttnWarps), kAttnThreads, smem, st>>>(a);
+	kernel<<<(unsigned)((p.items + kAttnWarps - 1) / kAttnWarps), kAttnThreads, smem, st>>>(a);
 	if (cudaError_t e = cudaGetLastError())
 		return e;
 	return launch_merge<T, HL, RPT>(a, p, st);
@@ -938,7 +979,7 @@ int moe_kv_attention(moe_kv_cache *cache, const moe_kv_batch *batch, const moe_r
 	auto plan_args = [&](const Plan &x, int64_t least, int64_t most) {
 		a.target = x.split ? x.target : 0;
 		a.items = x.items;
-		a.part = reinterpret_cast<float *>(part);
+		a.part = x.part_bytes ? reinterpret_cast<float *>(part) : nullptr;
 		a.part_rows = x.rows;
 		a.min_rows = (int)least;
 		a.max_rows = (int)most;

@@ -10,7 +10,14 @@ namespace kva {
 
 constexpr int kAttnTile = 32;      // key rows of a copy
 constexpr int kRunMin = 1;         // tiles of a run at least
-constexpr int kRunMax = 256;       // where runs are joined: 512 products in one fp32 chain
+constexpr int kRunMax = 256;       // where runs are joined
+// Key tiles (2 products each) of one chain of sums: the tensor cores cut what they add to a
+// sum, which costs it 1.4 (mma.sync) to 1.7 (tcgen05) units of 2^-23 a product, all of one sign
+// where the values are.  131072 rows in one chain were 7e-4 off; after kFold tiles the sums
+// move to the item's record in fp32 and begin anew: 256 products, below 2^-15.  Calls whose items
+// are shorter by their bounds take kernels without that (FOLD; with it a 2048-token prompt 135
+// us, without 127; 64 sequences 37.3 and 36.7).
+constexpr int kFold = 128;
 constexpr float kLag = 4.0f;       // exponents of 2 that the running maximum may lag (0: prompt 226 us, 196)
 constexpr float kLift = 10.0f;     // weights are held times 2^10
 constexpr float kNoMax = 3.0e38f;  // the bias kLift - m before any row was seen
@@ -46,7 +53,7 @@ struct AttnArgs {
 	int q_vec, o_vec;    // 16-byte aligned rows
 	int target;          // items wanted (0: one run a tile)
 	int64_t items;       // items that the workspace holds
-	float *part;         // [item][row][HL + 4]: sums, bias, weights' sum
+	float *part;         // records [item][row][HL + 4]: sums, bias, weights' sum; NULL: no item has one
 	int part_rows;       // rows of an item that can be in use
 	int min_rows, max_rows;   // query rows of a KV head in the sequences that are this kernel's
 };
@@ -419,6 +426,7 @@ struct Plan {
 	int64_t items = 0;       // and items
 	int target = 0;
 	bool split = false;      // runs at all
+	bool folds = false;      // items that may have more than kFold tiles
 	size_t part_bytes = 0;
 };
 

@@ -180,7 +180,7 @@ __device__ __forceinline__ void words_of(const uint8_t *p, uint32_t (&w)[NW])
 // products are 700 of the tensor cores', the rest is latency, of which the rows' steps
 // (a wait that finds its barrier done 200 to 300, scores 360, softmax 860, the hand-over
 // of P 330) and the issue of small products one after the other (120 each) are the most.
-template <typename T, int HL>
+template <typename T, int HL, bool FOLD>
 __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_constant__ AttnArgs a)
 {
 	using WL = WideLayout<HL>;
@@ -198,6 +198,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 		uint32_t shrinks, bads;
 		float shrink[NB];
 		uint32_t bad[NB];
+		float unit[NB];   // (tiles where sums move to the record) v_unit as of the tile
 	};
 	__shared__ Found found_s[2];
 	__shared__ float v_unit[NB];
@@ -473,6 +474,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 			} else if (tid == 0) {
 				found_s[i & 1].shrinks = found_s[i & 1].bads = 0;
 			}
+			if (FOLD && i % kFold == 0 && tid == 0)
+#pragma unroll
+				for (int b = 0; b < NB; b++)
+					found_s[i & 1].unit[b] = 1.0f / half_of(v_fac[b / 2], b & 1);
 		}
 		// 4 keys x 8 values: byte (block b0 or b0 + 1, value k or k + 1, and 16 further on)
 		const int g = lane % 8, w = tid / 8;
@@ -641,6 +646,43 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 			}
 			tmem_store_wait();
 		};
+		// the row's record: sums in true size, bias, weights' sum
+		float *pp = a.part + ((int64_t)blockIdx.x * a.part_rows + row) * (HL + 4);
+		// the sums of the tiles before to it, on top of what is there (!first)
+		auto fold = [&](bool first, const float *unit) {
+			float f = 0.0f;
+			if (row_used) {
+				if (!first) {
+					f = ex2(bias - pp[HL]);   // (the maximum only rises)
+					l = fmaf(pp[HL + 1], f, l);
+				}
+				*reinterpret_cast<float2 *>(pp + HL) = make_float2(bias, l);
+			}
+			l = 0.0f;
+#pragma unroll 1
+			for (int b = 0; b < NB; b++) {
+				uint32_t r[32];
+				const uint32_t at = tq + WL::kTmemO + 32 * b;
+				tmem_two(at, at + 16, r);
+				if (row_used) {
+#pragma unroll
+					for (int k = 0; k < 32; k += 4) {
+						float4 *d = reinterpret_cast<float4 *>(pp + 32 * b + k);
+						const float4 w = first ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : *d;
+						*d = make_float4(fmaf(w.x, f, __uint_as_float(r[k]) * unit[b]),
+								 fmaf(w.y, f, __uint_as_float(r[k + 1]) * unit[b]),
+								 fmaf(w.z, f, __uint_as_float(r[k + 2]) * unit[b]),
+								 fmaf(w.w, f, __uint_as_float(r[k + 3]) * unit[b]));
+					}
+				}
+#pragma unroll
+				for (int k = 0; k < 16; k++)
+					r[k] = 0;
+				tmem_store16(at, r);
+				tmem_store16(at + 16, r);
+			}
+			tmem_store_wait();
+		};
 		const float none = -__int_as_float(0x7f800000);
 		auto tile = [&](auto full_c, const float2 (&s)[kAttnTile / 2], int i, uint32_t seen) {
 			constexpr bool FULL = decltype(full_c)::value;   // every row sees all of it
@@ -689,13 +731,16 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 			sum[0] = add2(sum[0], sum[1]);
 			l += sum[0].x + sum[0].y;
 			// (P's place is free: S of this tile came after O += P V of tile i - 2)
-			if (i > 0 && (raise || fd.shrinks)) {
+			const bool folds = FOLD && i > 0 && i % kFold == 0;
+			if (i > 0 && (raise || fd.shrinks || folds)) {
 				wait(&bar_o[group][(i - 1) & 1], (i - 1) / 2);
 				fence_after();
 				if (fd.shrinks)   // V's factors of this tile
 					rescale(1.0f, fd.shrink);
 				if (raise)
 					rescale(f, nullptr);
+				if (folds)
+					fold(i == kFold, fd.unit);
 			}
 			if (fd.bads)
 #pragma unroll
@@ -749,8 +794,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 		if (ntile > 0)
 			wait(&bar_o[group][(ntile - 1) & 1], (ntile - 1) / 2);
 		fence_after();
+		const bool folded = FOLD && ntile > kFold;
+		float f = 0.0f;
+		if (folded && row_used) {
+			f = ex2(bias - pp[HL]);
+			l = fmaf(pp[HL + 1], f, l);
+		}
 		const RowOut<T> out(a, it, row, bias, l);
-		float *pp = a.part + ((int64_t)blockIdx.x * a.part_rows + row) * (HL + 4);
 #pragma unroll 1
 		for (int b = 0; b < NB; b++) {
 			uint32_t r[32];
@@ -770,8 +820,15 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 #pragma unroll
 				for (int k = 0; k < 8; k++)
 					v[k] = __uint_as_float(r[e + k]) * iv;
+				float4 *d = reinterpret_cast<float4 *>(pp + 32 * b + e);
+				if (folded) {
+					const float4 x = d[0], y = d[1];
+					const float w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+					for (int k = 0; k < 8; k++)
+						v[k] = fmaf(w[k], f, v[k]);
+				}
 				if (it.runs > 1) {
-					float4 *d = reinterpret_cast<float4 *>(pp + 32 * b + e);
 					d[0] = make_float4(v[0], v[1], v[2], v[3]);
 					d[1] = make_float4(v[4], v[5], v[6], v[7]);
 				} else {
@@ -798,9 +855,10 @@ template <typename T, int HL>
 cudaError_t launch_wide_as(const AttnArgs &a, const Plan &p, cudaStream_t st)
 {
 	constexpr int smem = WideLayout<HL>::kSmem;
-	if (cudaError_t e = ensure_smem(kv_wide_kernel<T, HL>, smem))
+	auto kernel = p.folds ? kv_wide_kernel<T, HL, true> : kv_wide_kernel<T, HL, false>;
+	if (cudaError_t e = ensure_smem(kernel, smem))
 		return e;
-	kv_wide_kernel<T, HL><<<(unsigned)p.items, kWideThreads, smem, st>>>(a);
+	kernel<<<(unsigned)p.items, kWideThreads, smem, st>>>(a);
 	if (cudaError_t e = cudaGetLastError())
 		return e;
 	return launch_merge<T, HL, kWideRows>(a, p, st);

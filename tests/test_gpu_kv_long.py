@@ -181,3 +181,99 @@ def test_attention_reports_every_sequence(m, dtype, q_len, kv, B):
     c.dev[0][B - 1] -= 1   # a query more for the last sequence than max_q
     c.attend(q)
     assert c.cache.status() == -1 and c.cache.status() == 0
+
+
+def long_rows(m, n, D, KVH, P, k, v):
+    """a cache of one sequence of n rows, its page table, and the rows that it holds"""
+    cache = m.KVCache(n // P, P, KVH, D)
+    table = torch.randperm(n // P, generator=torch.Generator().manual_seed(1)).to(torch.int32).cuda()[None]
+    one = [cuda_i32([0, n]), cuda_i32([n])]
+    b = m.KVBatch(1, n, n, n, one[0].data_ptr(), one[1].data_ptr(), table.data_ptr(), n // P)
+    cache.append(b, rows(m, k), rows(m, v), stream=LEGACY)
+    cache.gather(b, rows(m, k), rows(m, v), stream=LEGACY)
+    return cache, table, k, v
+
+
+def attend_long(m, cache, table, q, q_len, B, n, causal):
+    """B sequences over the same n rows"""
+    T, H, D = q.shape
+    tables = table.expand(B, -1).contiguous()
+    dev = [torch.arange(0, T + 1, q_len, dtype=torch.int32, device="cuda"),
+           torch.full((B,), n, dtype=torch.int32, device="cuda")]
+    b = m.KVBatch(B, T, q_len, n, *[x.data_ptr() for x in dev], tables.data_ptr(), table.shape[1])
+    out, lse = torch.empty_like(q), torch.empty(T, H, device="cuda")
+    size = cache.workspace_bytes(b, H)
+    ws = torch.full((max(size, 16),), 255, dtype=torch.uint8, device="cuda")
+    cache.attention(b, rows(m, q), rows(m, out), D ** -0.5, causal=causal, lse=lse.data_ptr(),
+                    workspace=ws.data_ptr(), workspace_bytes=size, stream=LEGACY)
+    assert cache.status() == 0
+    return out, lse
+
+
+MANY_ITEMS = [("f32", 64, 8, 1200, 1), ("f16", 64, 8, 1, 1200), ("f16", 64, 8, 2400, 1)]   # whole rows an item
+LONG_RUNS = [("f32", 64, 2, 1, 256), ("f16", 64, 8, 300, 1)]                               # runs of 256 tiles
+
+
+@pytest.mark.parametrize("dtype,D,G,q_len,B", MANY_ITEMS + LONG_RUNS)
+def test_attention_unsplit_long_rows(m, dtype, D, G, q_len, B):
+    """131072 rows in items of thousands of tiles, values of one sign: the tensor cores cut what
+    they add to a sum, 2 units of 2^-23 a product at most where 16 addends are each cut 3 bits
+    below it, so a chain of N of them loses up to N units of the last sum, half of it on the way
+    there.  Chains end after 256 products whatever the rows: 2^-15, and weights as in
+    attention_bounds (2^-19).  16-bit results are compared by the mean of their relative errors: each is
+    off by up to half of eps, evenly; there are 8 * 64 independent ones, so the mean of these is
+    off by eps / 2 / sqrt(3 * 512) and, at 5 deviations, by eps / 15."""
+    KVH, n, P = 8, 131072, 256
+    dt = TYPES[dtype]
+    g = torch.Generator(device="cuda").manual_seed(2)
+    k = torch.randn(n, KVH, D, device="cuda", generator=g)
+    v = torch.rand(n, KVH, D, device="cuda", generator=g) + torch.rand(1, KVH, D, device="cuda", generator=g)
+    cache, table, k, v = long_rows(m, n, D, KVH, P, k, v)
+    T = q_len * B
+    q = (torch.randn(T, KVH * G, D, device="cuda", generator=g) * 0.1).to(dt)
+    out, lse = attend_long(m, cache, table, q, q_len, B, n, False)
+    tokens = torch.tensor([0, 7, T // 2, T - 1], device="cuda")
+    rel, dl = [], []
+    for h in range(KVH):
+        kk, vv = k[:, h].double(), v[:, h].double()
+        x = q[tokens][:, h * G:(h + 1) * G].double()
+        s = torch.einsum("tgd,sd->tgs", x, kk).mul_(D ** -0.5)
+        want = torch.einsum("tgs,sd->tgd", s.softmax(-1), vv)
+        rel.append((out[tokens][:, h * G:(h + 1) * G].double() - want) / want)
+        dl.append((lse[tokens][:, h * G:(h + 1) * G].double() - s.logsumexp(-1)).abs().max())
+    rel = torch.cat(rel, 1)
+    assert max(dl) <= 2.0 ** -15
+    if dtype == "f32":
+        assert rel.abs().max() <= 2.0 ** -15 + 2.0 ** -18, rel.abs().max()
+    else:
+        eps = torch.finfo(dt).eps
+        assert rel.mean().abs() <= 2.0 ** -15 + 2.0 ** -18 + eps / 15, rel.mean()
+        assert rel.abs().max() <= 2.0 ** -15 + 2.0 ** -11 + eps / 2 * 1.01, rel.abs().max()
+
+
+@pytest.mark.parametrize("rising", [True, False])
+@pytest.mark.parametrize("dtype,D,G,q_len,B", MANY_ITEMS + [("bf16", 128, 8, 2400, 1), ("bf16", 256, 8, 1200, 1)])
+def test_attention_unsplit_growth(m, dtype, D, G, q_len, B, rising):
+    """items of 384 tiles whose sums move to their records on the way, while the scores and
+    V's scales grow (or fall) along the rows"""
+    KVH, n, P = 8, 12288, 64
+    g = torch.Generator(device="cuda").manual_seed(3)
+    at = torch.arange(n, device="cuda", dtype=torch.float32)
+    at = (at if rising else at.flip(0))[:, None, None]
+    k = torch.randn(n, KVH, D, device="cuda", generator=g)
+    k[..., :1] = at / 512 - 12
+    v = torch.randn(n, KVH, D, device="cuda", generator=g) * 2.0 ** torch.floor(at / 1000 - 9)
+    cache, table, k, v = long_rows(m, n, D, KVH, P, k, v)
+    T = q_len * B
+    q = torch.randn(T, KVH * G, D, device="cuda", generator=g)
+    q[..., 0] = torch.tensor([4.0, -3.0, 0.02, 1.0] * (KVH * G // 4), device="cuda")
+    q = q.to(TYPES[dtype])
+    out, lse = attend_long(m, cache, table, q, q_len, B, n, True)
+    k, v, x, o, l = f64(k), f64(v), f64(q), f64(out), f64(lse)
+    for t in (0, 31, T // 2, T - 1):
+        seen = n - q_len + t % q_len + 1
+        want, wl, size = ref.attention(x[t:t + 1], k[:seen], v[:seen], D ** -0.5)
+        tol, tol_l = ref.attention_bounds(q.dtype, size, np.abs(v[:seen]).max(), min(seen, 4096), want, wl)
+        err = np.abs(o[t:t + 1] - want)
+        assert (err <= tol).all(), f"token {t}: {(err / tol).max():.3g} of its bound"
+        assert (np.abs(l[t:t + 1] - wl) <= tol_l).all(), f"token {t}: lse"
