@@ -1508,7 +1508,7 @@ int change_kv(moe_model *m, int type)
 	if (!m->kvq) {
 		MRC(dalloc(m, &v, (size_t)(m->L * n * pb)));
 		m->kvq = static_cast<uint8_t *>(v);
-		MCK(cudaMemset(v, 0, (size_t)(m->L * n * pb)));
+		MCK(cudaMemsetAsync(v, 0, (size_t)(m->L * n * pb), m->st));
 	}
 	if (!m->kv_table) {
 		std::vector<int32_t> table((size_t)n);
@@ -1516,7 +1516,8 @@ int change_kv(moe_model *m, int type)
 			table[(size_t)i] = (int32_t)i;
 		MRC(dalloc(m, &v, (size_t)n * 4));
 		m->kv_table = static_cast<int32_t *>(v);
-		MCK(cudaMemcpy(v, table.data(), (size_t)n * 4, cudaMemcpyHostToDevice));
+		MCK(cudaMemcpyAsync(v, table.data(), (size_t)n * 4, cudaMemcpyHostToDevice, m->st));
+		MCK(cudaStreamSynchronize(m->st));   // `table` ends here
 	}
 	if (!m->kv_rope) {
 		moe_rope_desc r{};
@@ -1775,7 +1776,10 @@ int warm_up(moe_model *m)
 	if (e != cudaSuccess)
 		return mcuda(e, "moe_model: warm-up");
 	MRC(take_state_error(m));
-	MCK(cudaMemset(m->state, 0, S_WORDS * 4));
+	// on the model's stream, which the legacy stream does not order: the next call's state
+	// comes behind it
+	MCK(cudaMemsetAsync(m->state, 0, S_WORDS * 4, m->st));
+	MCK(cudaStreamSynchronize(m->st));
 	return MOE_OK;
 }
 
@@ -1908,7 +1912,11 @@ int moe_model_create(moe_model **out, const moe_model_desc *desc)
 			return rc;
 		}
 	}
-	rc = warm_up(m);
+	// what was set and copied above went through the legacy stream
+	{
+		const cudaError_t e = cudaDeviceSynchronize();
+		rc = e == cudaSuccess ? warm_up(m) : mcuda(e, "moe_model_create");
+	}
 	if (rc != MOE_OK) {
 		free_model(m);
 		return rc;

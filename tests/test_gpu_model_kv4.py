@@ -15,8 +15,11 @@ step; with a step of 0.27 rms (an eighth of a block's largest of 32 normal value
 3.3e-3 of the cached keys and of the values, each.  An attention output moves by
 about as much for either (a score's spread is 1), sqrt(2) * 3.3e-3 = 4.7e-3, and a
 final row by no more: rel-L2 5e-3."""
+import threading
+
 import numpy as np
 import pytest
+import torch
 
 from test_gguf import gguf_module
 
@@ -123,3 +126,41 @@ def test_refusals(moe, tmp_path):
         model.prefill([1], [64])
     model.prefill([1, 2], rows=False)
     assert model.status() == 0 and moe.lib().moe_model_set_kv(None, 0) == -1
+
+
+def test_set_kv_beside_other_work(moe, tmp_path):
+    """the cache's type changed while another thread keeps the legacy stream busy: the calls
+    behind it start from what set_kv left, bit for bit"""
+    model = build(moe, tmp_path, "olmoe", 2048, 256)
+    tok = np.random.default_rng(5).integers(0, 512, 40)
+
+    def calls():
+        got = []
+        for kind in (moe.Q4_0, moe.F32):
+            model.reset()
+            model.set_kv(kind)
+            got += [model.prefill(tok[:39]), model.decode(int(tok[39]), 39)]
+            model.reset()
+            model.set_kv(moe.Q4_0 if kind == moe.F32 else moe.F32)
+            got.append(model.decode(int(tok[0]), 0))
+        assert model.status() == 0
+        return got
+
+    quiet = calls()
+    stop = threading.Event()
+
+    def work():
+        a = torch.randn(2048, 2048, device="cuda", dtype=torch.bfloat16)
+        while not stop.is_set():
+            for _ in range(20):
+                a @ a
+            torch.cuda.current_stream().synchronize()
+
+    t = threading.Thread(target=work)
+    t.start()
+    try:
+        for _ in range(4):
+            assert all(np.array_equal(x, y) for x, y in zip(calls(), quiet))
+    finally:
+        stop.set()
+        t.join()
