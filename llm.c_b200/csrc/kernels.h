@@ -376,10 +376,10 @@ cudaError_t launch_kv_move_q4(uint8_t *pages, int64_t layer_bytes, int64_t page_
 			      int KVH, int HL, int page_log2, int from, int to, int rows,
 			      cudaStream_t st);
 
-// greedy pick (main.c:189-193: the first maximum) of logits [V] into
-// state[0] and picks[state[6] % pick_cap] (state[6] counts the picks); with
-// advance, the decode state {tok, pos, size, model_pos} moves one row on, and
-// state[7] (the rows of the cache with the next step's) with it
+// greedy pick (main.c:189-193: the first maximum) of logits [V] into the
+// model's state (its token, and picks[step % pick_cap], step counting the
+// picks); with advance, position, cache size and model position move one row
+// on, and the rows of the cache with the next step's with them
 // (scratch: device, at least 4 KB, zero before the first call)
 cudaError_t launch_argmax_advance(const float *logits, int V, int C, int32_t *state,
 				  int32_t *picks, int pick_cap, int advance, float *scratch,

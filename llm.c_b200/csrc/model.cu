@@ -16,6 +16,18 @@
 #include <float.h>
 #include <stdlib.h>
 
+namespace {
+
+// device state words; the first S_HOST are the host's to write in one copy
+// S_KV: cache rows with the call's own (4-bit cache: kv_len); S_QS: q_start of a
+// prefill (0, T), S_Q1: of a decode step (0, 1)
+// S_ERR: bits 1 (token id) and 2 (position / cache row) of this file's
+// kernels; S_PERR: the projections' bounded waits; S_STEP: picks made
+enum { S_TOK = 0, S_POS = 1, S_SIZE = 2, S_MPOS = 3, S_KV = 4, S_QS = 5, S_Q1 = 7, S_HOST = 9,
+       S_ERR = 9, S_PERR = 10, S_STEP = 11, S_WORDS = 12 };
+
+}  // namespace
+
 namespace moe {
 
 namespace {
@@ -758,15 +770,15 @@ argmax_advance_kernel(const float *logits, int V, int C, int32_t *state, int32_t
 	if (threadIdx.x == 0) {
 		*cnt = 0;
 		const int tok = idx < 0 ? 0 : idx;
-		state[0] = tok;
-		picks[state[6] % pick_cap] = tok;
-		state[6] += 1;
+		state[S_TOK] = tok;
+		picks[state[S_STEP] % pick_cap] = tok;
+		state[S_STEP] += 1;
 		if (advance) {
-			const int size = state[2] + 1, mpos = state[3] + 1;
-			state[2] = size;
-			state[3] = mpos;
-			state[1] = mpos >= C ? size : mpos;
-			state[7] = size + 1;
+			const int size = state[S_SIZE] + 1, mpos = state[S_MPOS] + 1;
+			state[S_SIZE] = size;
+			state[S_MPOS] = mpos;
+			state[S_POS] = mpos >= C ? size : mpos;
+			state[S_KV] = size + 1;
 		}
 	}
 }
@@ -983,13 +995,6 @@ int64_t row_bytes_of(int type, int64_t cols)
 	return type == MOE_F32 ? cols * 4 : cols / 32 * (type == MOE_Q8_0 ? Q8_0_BYTES : Q4_0_BYTES);
 }
 
-// device state words
-// S_ERR: bits 1 (token id) and 2 (position / cache row) of this file's
-// kernels; S_PERR: the projections' bounded waits; S_STEP: picks made
-// S_KV: cache rows with the call's own (4-bit cache: kv_len); S_QS: q_start of a
-// prefill (0, T), S_Q1: of a decode step (0, 1)
-enum { S_TOK = 0, S_POS = 1, S_SIZE = 2, S_MPOS = 3, S_ERR = 4, S_PERR = 5, S_STEP = 6, S_KV = 7,
-       S_QS = 8, S_Q1 = 10, S_WORDS = 12 };
 constexpr int64_t kKvPage = 64;   // rows of a page of the 4-bit cache
 
 }  // namespace
@@ -1342,18 +1347,13 @@ int write_state(moe_model *m, int64_t pos, int tok, int64_t T)
 	m->hstate[S_POS] = (int32_t)pos;
 	m->hstate[S_SIZE] = (int32_t)m->size;
 	m->hstate[S_MPOS] = (int32_t)m->mpos;
-	if (tok >= 0)
-		MCK(cudaMemcpyAsync(m->state, m->hstate, 4 * sizeof(int32_t), cudaMemcpyHostToDevice,
-				    m->st));
-	else
-		MCK(cudaMemcpyAsync(m->state + S_POS, m->hstate + S_POS, 3 * sizeof(int32_t),
-				    cudaMemcpyHostToDevice, m->st));
 	m->hstate[S_KV] = (int32_t)(m->size + T);
 	m->hstate[S_QS] = 0;
 	m->hstate[S_QS + 1] = (int32_t)T;
 	m->hstate[S_Q1] = 0;
 	m->hstate[S_Q1 + 1] = 1;
-	MCK(cudaMemcpyAsync(m->state + S_KV, m->hstate + S_KV, (S_WORDS - S_KV) * sizeof(int32_t),
+	const int from = tok >= 0 ? S_TOK : S_POS;
+	MCK(cudaMemcpyAsync(m->state + from, m->hstate + from, (S_HOST - from) * sizeof(int32_t),
 			    cudaMemcpyHostToDevice, m->st));
 	// the pinned words may be rewritten by the next call before this copy ran
 	MCK(cudaStreamSynchronize(m->st));
