@@ -6,6 +6,8 @@
 #include <cuda_fp16.h>
 
 struct moe_layer;  // include/moe_b200.h
+struct moe_kv_cache;
+struct moe_kv_desc;
 
 namespace moe {
 
@@ -370,6 +372,10 @@ bool pdl_enabled();
 // of each token RMS-normed over the whole vector
 cudaError_t launch_qk_norm(float *qkv, const float *q_norm, const float *k_norm, int T, int nq,
 			   int nk, float eps, cudaStream_t st);
+// kvcache.cu: moe_kv_create with an error word of the caller's (device memory, zero; NULL: its
+// own), and what the bits of such a word say
+int kv_create(::moe_kv_cache **out, const ::moe_kv_desc *desc, int32_t *err);
+int kv_status(const char *what, int32_t err);
 // kvcache.cu: rows [from, from + rows) -> [to, ..) of every layer's 4-bit pages (row r in
 // page r / page_size of its layer; the ranges do not overlap)
 cudaError_t launch_kv_move_q4(uint8_t *pages, int64_t layer_bytes, int64_t page_bytes, int L,

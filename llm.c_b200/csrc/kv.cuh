@@ -33,6 +33,7 @@ struct moe_kv_cache {
 	uint8_t *pages = nullptr;
 	bool owned = false;
 	int32_t *err = nullptr;
+	bool err_owned = false;
 };
 
 namespace moe {

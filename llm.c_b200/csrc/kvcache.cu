@@ -480,21 +480,7 @@ cudaError_t launch_kv_move_q4(uint8_t *pages, int64_t layer_bytes, int64_t page_
 	return cudaGetLastError();
 }
 
-}  // namespace moe
-
-using namespace moe;
-
-extern "C" {
-
-size_t moe_kv_page_bytes(int64_t page_size, int64_t n_kv_heads, int64_t head_len, int qtype)
-{
-	if (page_log2_of(page_size) < 0 || n_kv_heads <= 0 || n_kv_heads > 4096 ||
-	    (head_len != 64 && head_len != 128 && head_len != 256) || qtype != MOE_Q4_0)
-		return 0;
-	return (size_t)(2 * n_kv_heads * page_size * (head_len / 2 + head_len / 16));
-}
-
-int moe_kv_create(moe_kv_cache **out, const moe_kv_desc *desc)
+int kv_create(moe_kv_cache **out, const moe_kv_desc *desc, int32_t *err)
 {
 	const char *what = "moe_kv_create";
 	if (!out || !desc)
@@ -521,10 +507,13 @@ int moe_kv_create(moe_kv_cache **out, const moe_kv_desc *desc)
 	c->page_bytes = pb;
 	c->pages = static_cast<uint8_t *>(d.pages);
 	cudaError_t e = cudaGetDevice(&c->device);
-	if (e == cudaSuccess)
+	c->err = err;
+	if (e == cudaSuccess && !err) {
 		e = cudaMalloc(&c->err, 256);
-	if (e == cudaSuccess)
-		e = cudaMemset(c->err, 0, 256);
+		c->err_owned = e == cudaSuccess;
+		if (c->err_owned)
+			e = cudaMemset(c->err, 0, 256);
+	}
 	if (e == cudaSuccess && !c->pages) {
 		e = cudaMalloc(&c->pages, (size_t)d.n_pages * pb);
 		c->owned = e == cudaSuccess;
@@ -541,6 +530,37 @@ int moe_kv_create(moe_kv_cache **out, const moe_kv_desc *desc)
 	return MOE_OK;
 }
 
+int kv_status(const char *what, int32_t e)
+{
+	if (!e)
+		return MOE_OK;
+	if (e & kKvErrWait)
+		return kv_fail(MOE_ERR_TIMEOUT, "%s: a bounded wait in the attention kernel expired", what);
+	return kv_fail(MOE_ERR_INVALID, "%s:%s%s%s", what,
+		       e & kKvErrBatch ? " q_start or kv_len out of range;" : "",
+		       e & kKvErrPage ? " page outside the cache;" : "",
+		       e & kKvErrPos ? " position out of range;" : "");
+}
+
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" {
+
+size_t moe_kv_page_bytes(int64_t page_size, int64_t n_kv_heads, int64_t head_len, int qtype)
+{
+	if (page_log2_of(page_size) < 0 || n_kv_heads <= 0 || n_kv_heads > 4096 ||
+	    (head_len != 64 && head_len != 128 && head_len != 256) || qtype != MOE_Q4_0)
+		return 0;
+	return (size_t)(2 * n_kv_heads * page_size * (head_len / 2 + head_len / 16));
+}
+
+int moe_kv_create(moe_kv_cache **out, const moe_kv_desc *desc)
+{
+	return kv_create(out, desc, nullptr);
+}
+
 int moe_kv_destroy(moe_kv_cache *c)
 {
 	if (!c)
@@ -548,7 +568,8 @@ int moe_kv_destroy(moe_kv_cache *c)
 	DeviceGuard g(c->device);
 	cudaError_t e = g.e;
 	if (e == cudaSuccess) {
-		e = cudaFree(c->err);
+		if (c->err_owned)
+			e = cudaFree(c->err);
 		if (c->owned) {
 			const cudaError_t e2 = cudaFree(c->pages);
 			e = e == cudaSuccess ? e2 : e;
@@ -675,12 +696,7 @@ int moe_kv_status(moe_kv_cache *cache)
 		return MOE_OK;
 	KV_CK(what, cudaMemset(cache->err, 0, 4));
 	KV_CK(what, cudaDeviceSynchronize());   // before a call on any stream records the next
-	if (e & kKvErrWait)
-		return kv_fail(MOE_ERR_TIMEOUT, "%s: a bounded wait in the attention kernel expired", what);
-	return kv_fail(MOE_ERR_INVALID, "%s:%s%s%s", what,
-		       e & kKvErrBatch ? " q_start or kv_len out of range;" : "",
-		       e & kKvErrPage ? " page outside the cache;" : "",
-		       e & kKvErrPos ? " position out of range;" : "");
+	return kv_status(what, e);
 }
 
 }  // extern "C"

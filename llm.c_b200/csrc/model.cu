@@ -22,9 +22,10 @@ namespace {
 // S_KV: cache rows with the call's own (4-bit cache: kv_len); S_QS: q_start of a
 // prefill (0, T), S_Q1: of a decode step (0, 1)
 // S_ERR: bits 1 (token id) and 2 (position / cache row) of this file's
-// kernels; S_PERR: the projections' bounded waits; S_STEP: picks made
+// kernels; S_PERR: the projections' bounded waits; S_KVERR: every layer's
+// 4-bit cache; S_STEP: picks made
 enum { S_TOK = 0, S_POS = 1, S_SIZE = 2, S_MPOS = 3, S_KV = 4, S_QS = 5, S_Q1 = 7, S_HOST = 9,
-       S_ERR = 9, S_PERR = 10, S_STEP = 11, S_WORDS = 12 };
+       S_ERR = 9, S_PERR = 10, S_KVERR = 11, S_STEP = 12, S_WORDS = 13 };
 
 }  // namespace
 
@@ -1448,18 +1449,18 @@ int capture(moe_model *m)
 int take_state_error(moe_model *m)
 {
 	MCK(cudaStreamSynchronize(m->st));
-	int32_t e[2] = {0, 0};
-	MCK(cudaMemcpy(e, m->state + S_ERR, 8, cudaMemcpyDeviceToHost));
-	if (e[0] || e[1]) {
-		MCK(cudaMemset(m->state + S_ERR, 0, 8));
+	int32_t e[3] = {0, 0, 0};
+	MCK(cudaMemcpyAsync(e, m->state + S_ERR, sizeof e, cudaMemcpyDeviceToHost, m->st));
+	MCK(cudaStreamSynchronize(m->st));
+	if (e[0] || e[1] || e[2]) {
+		MCK(cudaMemsetAsync(m->state + S_ERR, 0, sizeof e, m->st));
 		if (e[1])
 			return mfail(MOE_ERR_TIMEOUT, "moe_model: a bounded wait expired in a projection");
+		if (!e[0])
+			return moe::kv_status("moe_model", e[2]);
 		return mfail(MOE_ERR_INVALID, "moe_model: %s%s", (e[0] & 1) ? "token id outside the "
 			     "vocabulary; " : "", (e[0] & 2) ? "position or cache row out of range" : "");
 	}
-	// every layer's cache meets the same lengths, pages and positions
-	if (!m->kvl.empty())
-		MRC(moe_kv_status(m->kvl[0]));
 	for (const auto &ly : m->layers)
 		if (ly.moe)
 			MRC(moe_layer_status(ly.moe));
@@ -1531,7 +1532,7 @@ int change_kv(moe_model *m, int type)
 		const int64_t l = (int64_t)m->kvl.size();
 		moe_kv_desc d{n, kKvPage, m->KVH, m->HL, MOE_Q4_0, m->kvq + l * n * pb};
 		moe_kv_cache *c;
-		MRC(moe_kv_create(&c, &d));
+		MRC(moe::kv_create(&c, &d, m->state + S_KVERR));
 		m->kvl.push_back(c);
 	}
 	if (!m->kv_ws1) {
