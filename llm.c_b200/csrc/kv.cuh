@@ -123,11 +123,12 @@ inline int check_rows(const char *what, const char *name, const moe_rows *r, int
 		// other dimension's extent
 		const bool t1 = n_tokens <= 1, h1 = r->n_heads == 1;
 		const int64_t over_h = (r->n_heads - 1) * hs + head_len;
-		const int64_t over_t = (n_tokens > 0 ? n_tokens - 1 : 0) * ts + head_len;
 		const bool ok = t1 && h1 ? true
 				: t1 ? hs >= head_len
 				: h1 ? ts >= head_len
-				     : (hs >= head_len && ts >= over_h) || (ts >= head_len && hs >= over_t);
+				     // (the tokens' extent may pass 64 bits)
+				     : (hs >= head_len && ts >= over_h) ||
+				       (ts >= head_len && hs >= head_len && n_tokens - 1 <= (hs - head_len) / ts);
 		if (!ok)
 			return kv_fail(MOE_ERR_INVALID, "%s: rows of %s overlap (strides %lld, %lld)", what,
 				       name, (long long)ts, (long long)hs);

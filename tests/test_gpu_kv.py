@@ -185,6 +185,23 @@ def test_rope_refusals(m):
     assert r.status() == 0
 
 
+def test_rope_refuses_rows_past_64_bits(m):
+    """tokens times their stride beyond 64 bits: rows of one place for all heads are refused"""
+    r = m.Rope(64, 1e4, 100)
+    x, pos = rand(1, 4, 2, 64).cuda(), cuda_i32([1] * 4)
+    for n, ts, hs in (((1 << 23) + 1, 1 << 40, 0), (1 << 30, 1 << 40, 0), ((1 << 24) + 1, 1 << 40, 63),
+                      ((1 << 24) + 1, 1 << 38, 1 << 39)):
+        with pytest.raises(m.MoeError) as e:
+            r.forward(n, 64, pos.data_ptr(), rows(m, x), m.Rows(x.data_ptr(), m.F32, 2, ts, hs), stream=LEGACY)
+        assert e.value.code == -1
+    # head-major rows that just fit, and one value less
+    y = torch.empty(2 * 4 * 64, device="cuda")
+    r.forward(4, 64, pos.data_ptr(), rows(m, x), m.Rows(y.data_ptr(), m.F32, 2, 64, 256), stream=LEGACY)
+    with pytest.raises(m.MoeError):
+        r.forward(4, 64, pos.data_ptr(), rows(m, x), m.Rows(y.data_ptr(), m.F32, 2, 64, 255), stream=LEGACY)
+    assert r.status() == 0
+
+
 # ------------------------------------------------------------------ a batch and its cache
 class Case:
     """Sequences with random keys and values in a shuffled pool; `fill` "nan" puts a NaN
