@@ -162,6 +162,8 @@ inline int check_batch(const char *what, const moe_kv_cache *c, const moe_kv_bat
 	if (arrays && b->n_seqs > 0 && b->n_tokens > 0 &&
 	    (!b->q_start || !b->kv_len || (b->max_kv > 0 && !b->page_table)))
 		return kv_fail(MOE_ERR_INVALID, "%s: batch arrays missing", what);
+	if (arrays && ((uintptr_t)b->q_start | (uintptr_t)b->kv_len | (uintptr_t)b->page_table) % 4)
+		return kv_fail(MOE_ERR_INVALID, "%s: batch arrays are not aligned", what);
 	return MOE_OK;
 }
 

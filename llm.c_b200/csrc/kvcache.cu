@@ -597,6 +597,8 @@ int moe_kv_append(moe_kv_cache *cache, const moe_kv_batch *batch, const moe_rope
 	const int64_t T = batch->n_tokens, D = cache->d.head_len, KVH = cache->d.n_kv_heads;
 	if (!k || !v || (!q) != (!q_out))
 		return kv_fail(MOE_ERR_INVALID, "%s: k or v missing, or q without q_out", what);
+	if ((uintptr_t)pos % 4)
+		return kv_fail(MOE_ERR_INVALID, "%s: positions are not aligned", what);
 	if (rope && rope->device != cache->device)
 		return kv_fail(MOE_ERR_INVALID, "%s: rope and cache are on devices %d and %d", what,
 			       rope->device, cache->device);

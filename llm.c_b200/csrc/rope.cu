@@ -373,8 +373,8 @@ int moe_rope_forward(moe_rope *rope, int64_t n_tokens, int64_t head_len, const i
 		return rc;
 	if (n_tokens == 0)
 		return MOE_OK;
-	if (!pos)
-		return kv_fail(MOE_ERR_INVALID, "%s: positions missing", what);
+	if (!pos || (uintptr_t)pos % 4)
+		return kv_fail(MOE_ERR_INVALID, "%s: positions missing or not aligned", what);
 	cudaStream_t st;
 	if ((rc = resolve_stream(what, rope->device, stream, &st)) != MOE_OK)
 		return rc;

@@ -962,3 +962,28 @@ def test_own_pages_and_library_stream(m):
     m.check(m.lib().moe_sync())
     assert np.array_equal(out.cpu().numpy(), ref.values(*ref.quantize(k.cpu().numpy())))
     assert cache.status() == 0
+
+
+def test_unaligned_arrays_refused(m):
+    """positions, lengths and page tables off their 4 bytes are refused by every call"""
+    c = Case(m, [1, 1], [40, 50], 1, 64, 16)
+    x = rand(1, 2, 4, 64).cuda()
+    q, k = rows(m, x), rows(m, x[:, :1])
+    out = rows(m, torch.empty_like(x))
+    ws = torch.empty(max(16, c.cache.workspace_bytes(c.batch, 4)), dtype=torch.uint8, device="cuda")
+    pos, r = cuda_i32([1, 2, 3]), m.Rope(64, 1e4, 100)
+
+    def no(fn, *a, **kw):
+        with pytest.raises(m.MoeError) as e:
+            fn(*a, stream=LEGACY, **kw)
+        assert e.value.code == -1
+
+    for field in ("q_start", "kv_len", "page_table"):
+        b = type(c.batch).from_buffer_copy(c.batch)
+        setattr(b, field, getattr(b, field) + 2)
+        no(c.cache.attention, b, q, out, 0.1, workspace=ws.data_ptr(), workspace_bytes=ws.numel())
+        no(c.cache.append, b, k, k)
+        no(c.cache.gather, b, k)
+    no(c.cache.append, c.batch, k, k, rope=r, pos=pos.data_ptr() + 1)
+    no(r.forward, 2, 64, pos.data_ptr() + 2, q, out)
+    assert c.cache.status() == 0 and r.status() == 0
