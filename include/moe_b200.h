@@ -501,7 +501,7 @@ MOE_API int moe_kv_gather(moe_kv_cache *cache, const moe_kv_batch *batch, const 
  * of 2^13 or more; fp32 rows: q and weights as two fp16 halves, about 22 bits);
  * sums and softmax statistics are held in fp32 (below 256 query rows, 16-bit
  * rows' products enter a sum with about 17 bits; the tensor cores' sums are of 256
- * products of 16 rows at most, which stay within 2^-15 where all values have one
+ * products of 16 rows at most, which stay within 2^-14 where all values have one
  * sign, and are added up in fp32).  Rows that a query does not see never reach its
  * result, whatever they hold.
  * workspace: 16-byte aligned, at least moe_kv_attention_workspace bytes (which

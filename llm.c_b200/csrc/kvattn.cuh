@@ -11,12 +11,13 @@ namespace kva {
 constexpr int kAttnTile = 32;      // key rows of a copy
 constexpr int kRunMin = 1;         // tiles of a run at least
 constexpr int kRunMax = 256;       // where runs are joined
-// Key tiles (2 products each) of one chain of sums: the tensor cores cut what they add to a
-// sum, which costs it 1.4 (mma.sync) to 1.7 (tcgen05) units of 2^-23 a product, all of one sign
-// where the values are.  131072 rows in one chain were 7e-4 off; after kFold tiles the sums
-// move to the item's record in fp32 and begin anew: 256 products, below 2^-15.  Calls whose items
-// are shorter by their bounds take kernels without that (FOLD; with it a 2048-token prompt 135
-// us, without 127; 64 sequences 37.3 and 36.7).
+// Key tiles (2 products of 16 rows each) of one chain of sums: the tensor cores cut what they
+// add to a sum, always towards zero, so 131072 rows of one sign in one chain came out 6.8e-4
+// (mma.sync) and 8.3e-4 (tcgen05) too small.  After kFold tiles the sums move to the item's
+// record in fp32 and begin anew: 256 products, below 2^-14 (fp32 rows 1.8e-6 off).  131072 and
+// 8192 rows take 0.8 (kvattn.cu) and 2 to 4 (kvwide.cu) % longer so.  Calls whose items are
+// shorter by their bounds take kernels without that (FOLD): a 2048-token prompt 127 us, in the
+// first form with it 135; 64 sequences 36.7 and 37.3.
 constexpr int kFold = 128;
 constexpr float kLag = 4.0f;       // exponents of 2 that the running maximum may lag (0: prompt 226 us, 196)
 constexpr float kLift = 10.0f;     // weights are held times 2^10

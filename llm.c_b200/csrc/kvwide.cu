@@ -114,6 +114,14 @@ __device__ __forceinline__ void tmem_two(uint32_t a, uint32_t b, uint32_t (&r)[3
 		: KV_R16(r, 0), KV_R16(r, 16)
 		: "r"(a), "r"(b));
 }
+__device__ __forceinline__ void tmem_one(uint32_t a, uint32_t (&r)[16])
+{
+	asm volatile(
+		"tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+		"tcgen05.wait::ld.sync.aligned;"
+		: KV_R16(r, 0)
+		: "r"(a));
+}
 __device__ __forceinline__ void tmem_store16(uint32_t a, const uint32_t *r)
 {
 	asm volatile(
@@ -648,38 +656,38 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 		};
 		// the row's record: sums in true size, bias, weights' sum
 		float *pp = a.part + ((int64_t)blockIdx.x * a.part_rows + row) * (HL + 4);
-		// the sums of the tiles before to it, on top of what is there (!first)
-		auto fold = [&](bool first, const float *unit) {
-			float f = 0.0f;
-			if (row_used) {
-				if (!first) {
-					f = ex2(bias - pp[HL]);   // (the maximum only rises)
-					l = fmaf(pp[HL + 1], f, l);
-				}
-				*reinterpret_cast<float2 *>(pp + HL) = make_float2(bias, l);
+		// the sums of the tiles before to it, on top of what is there (!first): times f and the
+		// blocks' factors, in true size
+		auto fold = [&](bool first, float f, const float *blocks, const float *unit) {
+			float g = 0.0f;
+			if (!first && row_used) {
+				g = ex2(bias - pp[HL]);   // (the maximum only rises)
+				l = fmaf(pp[HL + 1], g, l);
 			}
+			if (row_used)
+				*reinterpret_cast<float2 *>(pp + HL) = make_float2(bias, l);
 			l = 0.0f;
 #pragma unroll 1
-			for (int b = 0; b < NB; b++) {
-				uint32_t r[32];
-				const uint32_t at = tq + WL::kTmemO + 32 * b;
-				tmem_two(at, at + 16, r);
+			for (int e = 0; e < HL; e += 16) {
+				uint32_t r[16];
+				const uint32_t at = tq + WL::kTmemO + e;
+				tmem_one(at, r);
+				const float u = f * unit[e / 32] * (blocks ? blocks[e / 32] : 1.0f);
 				if (row_used) {
 #pragma unroll
-					for (int k = 0; k < 32; k += 4) {
-						float4 *d = reinterpret_cast<float4 *>(pp + 32 * b + k);
+					for (int k = 0; k < 16; k += 4) {
+						float4 *d = reinterpret_cast<float4 *>(pp + e + k);
 						const float4 w = first ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : *d;
-						*d = make_float4(fmaf(w.x, f, __uint_as_float(r[k]) * unit[b]),
-								 fmaf(w.y, f, __uint_as_float(r[k + 1]) * unit[b]),
-								 fmaf(w.z, f, __uint_as_float(r[k + 2]) * unit[b]),
-								 fmaf(w.w, f, __uint_as_float(r[k + 3]) * unit[b]));
+						*d = make_float4(fmaf(w.x, g, __uint_as_float(r[k]) * u),
+								 fmaf(w.y, g, __uint_as_float(r[k + 1]) * u),
+								 fmaf(w.z, g, __uint_as_float(r[k + 2]) * u),
+								 fmaf(w.w, g, __uint_as_float(r[k + 3]) * u));
 					}
 				}
 #pragma unroll
 				for (int k = 0; k < 16; k++)
 					r[k] = 0;
 				tmem_store16(at, r);
-				tmem_store16(at + 16, r);
 			}
 			tmem_store_wait();
 		};
@@ -735,12 +743,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv_wide_kernel(const __grid_c
 			if (i > 0 && (raise || fd.shrinks || folds)) {
 				wait(&bar_o[group][(i - 1) & 1], (i - 1) / 2);
 				fence_after();
-				if (fd.shrinks)   // V's factors of this tile
-					rescale(1.0f, fd.shrink);
-				if (raise)
-					rescale(f, nullptr);
-				if (folds)
-					fold(i == kFold, fd.unit);
+				if (folds) {
+					fold(i == kFold, f, fd.shrinks ? fd.shrink : nullptr, fd.unit);
+				} else {
+					if (fd.shrinks)   // V's factors of this tile
+						rescale(1.0f, fd.shrink);
+					if (raise)
+						rescale(f, nullptr);
+				}
 			}
 			if (fd.bads)
 #pragma unroll
