@@ -29,7 +29,8 @@
 // below what rounding the output to bf16 costs and twice fp16's; fp32 rows take two
 // columns, the fp16 value of the fp32 product and the fp16 remainder.  q is brought
 // to 2^13 by a power of two per row, so that fp16 holds 16-bit rows' values exactly
-// unless they are 2^-27 of the row's largest.
+// unless they are below 2^-27 (those that meet high nibbles, which count 16-fold, 2^-23) of
+// the row's largest, and is off by 2^-38 (2^-34) of it where not.
 //
 // Work: an item is a KV head of a sequence, a tile of its query rows (query
 // token x head of the group) and a run of 32-row key tiles, and an item is a warp's:
@@ -97,7 +98,8 @@ __device__ __forceinline__ uint32_t smem_addr(const void *p)
 	return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
-// Codes as fp16 numbers, a pair from a word's low nibbles (bytes 0 and 2) or high ones.
+// Codes as fp16 numbers (the method of adding a code to the bits of a power of two is published:
+// Kim et al. 2022, arXiv 2211.10017), a pair from a word's low nibbles (bytes 0 and 2) or high ones.
 // 16-bit rows: masked out in place, subnormals code * 2^-24 and code * 2^-20, for one
 // logic operation; the -8 of a code is the caller's (RAW) or one exact subtraction more.
 // The tensor cores line sums up by a subnormal's nominal exponent, so these sums carry
@@ -174,9 +176,11 @@ template <int HL, int NT>
 constexpr int kAttnCtas = HL == 128 && NT == 1 ? 4 : 1;
 
 // grid: the plan's items, kAttnWarps to a CTA.  Few queries (4 sequences of 131072 rows,
-// 32 heads on 8: 526 MB in 124 us, 4.25 TB/s of 6.5) are bound by the instructions
-// that take codes apart, a batch of 64 such sequences of up to 4096 rows (72 MB in
-// 37 us) by latency: a few tiles a warp between its plan and its last store.
+// 32 heads on 8: 526 MB in 124 us, 4.25 TB/s of 6.5) are bound by chains
+// of dependent instructions that take codes apart (issue 63 %, ALU 55 %, 14 warps an SM), a batch
+// of 64 such sequences of up to 8192 rows (72 MB in 37 us) by latency: a few tiles a warp
+// between its plan and its last store.  (Times from CUDA graphs of calls; one call at a time
+// takes 2 to 3 us more.)
 template <typename T, int HL, int NT, bool FOLD>
 __global__ void __launch_bounds__(kAttnThreads, kAttnCtas<HL, NT>) kv_attn_kernel(AttnArgs a)
 {
@@ -838,7 +842,8 @@ Plans plan_of(const moe_kv_cache *c, const moe_kv_batch *b, int64_t H, bool fp32
 		// with 4: 196)
 		ps.n.nt = r <= per ? 1 : r <= 2 * per || HL == 256 ? 2 : 4;
 		ps.n.rpt = per * ps.n.nt;
-		// 16 resident warps an SM, fewer for wide tiles
+		// 16 resident warps an SM, fewer for wide tiles (at head length 64 the registers
+		// leave 8 to 12 of the 16)
 		plan_items(ps.n, c, b, G, r, (int64_t)sm_count() * kAttnWarps * (HL * ps.n.nt <= 128 ? 4 : 2));
 	}
 	if (ps.wide) {

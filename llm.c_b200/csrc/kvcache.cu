@@ -137,8 +137,8 @@ __device__ __forceinline__ void row_bytes(uint32_t word, int b, bool isv, uint32
 // tokens' sequences (a search of two rounds), angles and pages, each a dependent
 // load.  A lane has 8 values of a row and the same place in every row it meets, so a
 // token's angles stay in its registers (kTurnAny: halves that are no multiple of 8,
-// value by value).  64 decode tokens 8.0 us; 512 fp32 tokens of 16 + 32 heads 16.5; 16383 ragged
-// fp16 ones of 28 + 8 heads of 64 44 (72 % of the issue slots: maxima and bytes by
+// value by value).  64 decode tokens 4.9 us; 512 fp32 tokens of 16 + 32 heads 10.3; 16383 ragged
+// fp16 ones of 28 + 8 heads of 64 42.8 (72 % of the issue slots: maxima and bytes by
 // shuffles, a rounding a value).
 template <typename T, bool VEC, int TURN>
 __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) append_kernel(const __grid_constant__ AppendArgs<T> a)
