@@ -435,6 +435,7 @@ int layer_scratch(moe_layer *L, int64_t T)
 	L->gbar = (unsigned long long *)(b + o_gbar);
 	L->t1cnt = (unsigned *)(b + o_t1cnt);
 	L->stamps = (uint64_t *)(b + o_stamps);
+	CK(cudaMemset(L->err, 0, 4));
 	CK(cudaMemset(L->gbar, 0, gbar_bytes));
 	CK(cudaMemset(L->t1cnt, 0, 4));
 	CK(cudaDeviceSynchronize());  // ordered before launches on any stream

@@ -283,3 +283,19 @@ def test_config0_layer(moe, orc, olmoe, T):
     assert_dispatch(orc, ids, counts, offsets, perm, 64)
     assert_output_close(got, ref)
     lay.close()
+
+
+@pytest.mark.parametrize("T", [1, 3, 45, 300])
+def test_scratch_in_used_memory(moe, orc, small_layers, T):
+    """a layer whose scratch lies in memory that was written and freed before: its error word
+    starts from zero"""
+    L = small_layers[1]
+    x = orc.make_tokens(15, T, SMALL["d"])
+    ref = orc.moe_ffn(L, x)[0]
+    used = [moe.DeviceBuffer.from_numpy(np.full(n, 0x5b, np.uint8))
+            for n in [1 << k for k in range(15, 25)] for _ in range(6)]
+    lays = [build(moe, L) for _ in range(6)]
+    for b in used:
+        b.free()
+    for i, lay in enumerate(lays):
+        assert_output_close(lay.forward(x, flags=moe.SIMPLE if i % 2 else 0), ref)
