@@ -504,6 +504,8 @@ MOE_API int moe_kv_gather(moe_kv_cache *cache, const moe_kv_batch *batch, const 
  * products of 16 rows at most, which stay within 2^-14 where all values have one
  * sign, and are added up in fp32).  Rows that a query does not see never reach its
  * result, whatever they hold.
+ * Every item of work looks through all lengths of the batch first: some thousands
+ * of sequences a call, not more (1024 of 100 to 2000 rows: 0.43 ms).
  * workspace: 16-byte aligned, at least moe_kv_attention_workspace bytes (which
  * follow from n_heads, the cache and the batch's n_seqs, n_tokens, max_q and
  * max_kv; 0: none needed); what it holds counts for this call only. */
